@@ -54,7 +54,7 @@ enum { ONEBIT_KERNEL_AUTO = 0,    /* few-token kernel for n <= 16 (n <= 32 up to
        ONEBIT_KERNEL_STABLE_WEIGHTS = 0x100 };
 
 enum { ONEBIT_OK = 0, ONEBIT_ERR_SHAPE = 1, ONEBIT_ERR_NULL = 2, ONEBIT_ERR_CUDA = 3,
-       ONEBIT_ERR_WORKSPACE = 4, ONEBIT_ERR_ARG = 5, ONEBIT_ERR_DEVICE_WAIT = 6 };
+       ONEBIT_ERR_WORKSPACE = 4, ONEBIT_ERR_ARG = 5, ONEBIT_ERR_DEVICE_WAIT = 6, ONEBIT_ERR_BATCH = 7 };
 
 /* Message of the calling thread's most recent failed call ("" if none). Host pointer, valid until
  * the thread's next failing call. Replaces the reference's exit(EXIT_FAILURE) (csrc/kernel_lib.cu:11-20). */
@@ -198,9 +198,68 @@ int onebit_unpack_to_dense(const void *bits_tile, const void *meta_tile, const v
 int onebit_sparse_matmul_static(const void *a_bits, const void *b, void *d, const void *e_meta, const void *scale,
                                 int64_t m, int64_t n, int64_t k, int out_type, int meta_dialect, void *stream);
 
+/* ---- The operators between the linear layers of a decoder block -------------------------------------------------------
+ * No counterpart in the reference, whose model demo leaves them to the model (tests/python/test_model_replace.py:22-44).
+ * dtype: ONEBIT_DENSE_F16 or ONEBIT_DENSE_BF16, the type of every 16-bit tensor of the call. Strides are in elements; the
+ * innermost dimension is contiguous. Arithmetic, sums and statistics are fp32, rounded once at the store. */
+
+/* Residual add with the norms around it, row by row (rows x hidden, hidden <= ONEBIT_NORM_MAX_HIDDEN):
+ *   u = post_weight ? x / sqrt(mean(x^2) + eps) * post_weight : x
+ *   h = residual + residual_scale * gate * u        y = h / sqrt(mean(h^2) + eps) * weight
+ * gate: NULL, one row for all (gate_stride 0) or a row for each. residual and h are fp32 if residual_f32, else of dtype. With
+ * residual NULL, h = x is not written (and gate and post_weight must be NULL). y may be x, h may be residual. */
+#define ONEBIT_NORM_MAX_HIDDEN 32768
+int onebit_residual_norm(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, int residual_f32, const void *gate,
+                         int64_t gate_stride, const void *post_weight, const void *weight, void *y, int64_t y_stride, void *h,
+                         int64_t h_stride, int64_t rows, int64_t hidden, float residual_scale, float eps, int dtype, void *stream);
+
+/* Rotary positions of x (tokens, heads, head_dim <= ONEBIT_ROTARY_MAX_DIM): in the first rotary_dim values of every head, pair i
+ * (values i and i + rotary_dim / 2, or 2i and 2i + 1 if interleaved) is turned by positions[token] * inv_freq[i] and
+ * multiplied by magnitude; the other values pass through. inv_freq: rotary_dim / 2 doubles (device). positions: int32 or int64,
+ * any sign, no loss of precision at far positions. y may be x. */
+#define ONEBIT_ROTARY_MAX_DIM 512
+int onebit_rotary(const void *x, int64_t x_token_stride, int64_t x_head_stride, void *y, int64_t y_token_stride, int64_t y_head_stride,
+                  const void *positions, int positions_i64, const double *inv_freq, int rotary_dim, int interleaved, float magnitude,
+                  int64_t tokens, int64_t heads, int64_t head_dim, int dtype, void *stream);
+
+/* The 8-bit key/value cache. A page holds 64 tokens: k_pages (pages, kv_heads, 64, head_dim), v_pages (pages, kv_heads,
+ * head_dim, 64), both e4m3 bytes, 16-byte aligned; k_scale, v_scale (pages, kv_heads) fp32: a stored value stands for
+ * code * scale. head_dim 64 or 128. A batch (device int32): sequence s has the new tokens q_start[s] .. q_start[s+1] - 1 of the
+ * call's `tokens` rows and kv_len[s] tokens in the cache INCLUDING the new ones; the token at position p lies in page
+ * block_table[s * table_stride + p / 64]. Rows that belong to no sequence are neither read nor written. A page number outside
+ * [0, pages), a position beyond table_width pages or rows beyond `tokens` are skipped, and onebit_check_device_status
+ * reports ONEBIT_ERR_BATCH.
+ *
+ * onebit_cache_append turns k (as onebit_rotary at the tokens' own positions; rotary_dim 0: not at all) and stores k and v:
+ * the page's scale becomes the smallest power of two from 2^-32 to 2^32 that brings the new tokens' largest finite |value| to
+ * at most 448, but not less than the scale of tokens that the page held before the call; those are re-scaled if it grew. A page
+ * without earlier tokens gets zeros behind the new ones. Infinities are stored as the largest value, a NaN key value as NaN; a
+ * token with a NaN in v has it stored as 0 and its key made NaN. q (nullable, heads a multiple of kv_heads) is turned into q_out,
+ * which may be q. A page that is written may belong to one sequence of the batch only. */
+int onebit_cache_append(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                        const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                        const double *inv_freq, int rotary_dim, int interleaved, float magnitude, void *k_pages, void *v_pages,
+                        float *k_scale, float *v_scale, int64_t pages, const int *q_start, const int *kv_len, const int *block_table,
+                        int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                        int64_t head_dim, int dtype, void *stream);
+
+/* out (tokens, heads, head_dim) = softmax(scale * q k^T) v over each sequence's cache; head h reads cache head
+ * h / (heads / kv_heads). causal: a new token at position p sees the positions up to p (the new tokens are the last of
+ * kv_len), else all kv_len. A row that sees nothing gets zeros. q, out: 16-byte aligned, strides multiples of 8.
+ * max_new: the caller's bound of a sequence's new tokens (0: tokens); it only selects the kernel, results are right for any value.
+ * workspace: device memory of onebit_cache_attend_workspace bytes (may be 0), 256-byte aligned, for this call until its work on
+ * `stream` has finished. */
+size_t onebit_cache_attend_workspace(int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new);
+int onebit_cache_attend(const void *q, int64_t q_token_stride, int64_t q_head_stride, void *out, int64_t out_token_stride, int64_t out_head_stride,
+                        const void *k_pages, const void *v_pages, const float *k_scale, const float *v_scale, int64_t pages,
+                        const int *q_start, const int *kv_len, const int *block_table, int64_t table_stride, int64_t table_width,
+                        int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, float scale,
+                        int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Synchronises the current device, then reads and clears its status word: ONEBIT_ERR_DEVICE_WAIT if
  * a bounded wait inside the tensor-memory kernel gave up since the last call (the kernel then still
- * terminated, with an unusable result), ONEBIT_OK otherwise. The reference has no counterpart; its
+ * terminated, with an unusable result), ONEBIT_ERR_BATCH if a cache operator left out a page or rows that a batch named
+ * outside their range, ONEBIT_OK otherwise. The reference has no counterpart; its
  * kernel has no device-side waits on other agents. */
 int onebit_check_device_status(void);
 

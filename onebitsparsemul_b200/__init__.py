@@ -12,6 +12,8 @@ import torch.nn as nn
 from . import _lib
 from ._lib import (DENSE_BF16, DENSE_F16, DENSE_I32, KERNEL_AUTO, KERNEL_DECODE, KERNEL_PREFILL, KERNEL_STABLE_WEIGHTS,
                    META_CUTLASS, META_PYTHON, OUT_F16, OUT_F32, OneBitError)
+from .block_ops import (CacheBatch, KVCache8, cache_append, cache_attend, residual_norm, rotary_frequencies,
+                        rotary_tokens)
 from ._semi_structured_conversions import (mask_creator, sparse_semi_structured_from_dense_cutlass,
                                            sparse_semi_structured_to_dense_cutlass)
 
@@ -20,6 +22,7 @@ __all__ = [
     "py_binary_gemm", "BinaryLinear_2_4", "sparse_semi_structured_from_dense_cutlass",
     "sparse_semi_structured_to_dense_cutlass", "mask_creator", "PackedWeight", "pack_weight", "matmul_packed",
     "relayout", "matmul_rows", "matmul_scatter", "matmul_packed_host", "linear_tokens", "replace_linear_layers", "OneBitError",
+    "residual_norm", "rotary_frequencies", "rotary_tokens", "KVCache8", "CacheBatch", "cache_append", "cache_attend",
 ]
 
 

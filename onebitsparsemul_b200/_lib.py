@@ -18,7 +18,7 @@ KERNEL_AUTO, KERNEL_PREFILL, KERNEL_DECODE = 0, 1, 2
 KERNEL_STABLE_WEIGHTS = 0x100     # flag OR-ed into a kernel selector (see the header)
 
 # every extern "C" symbol of include/onebit_sparse_tensor.h, with its ctypes signature
-_vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+_vp, _i64, _int, _sz, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 SIGNATURES = {
     "onebit_last_error": (ctypes.c_char_p, []),
     "onebit_packed_bits_bytes": (_sz, [_i64, _i64]),
@@ -38,6 +38,12 @@ SIGNATURES = {
     "onebit_mask24": (_int, [_vp, _i64, _vp, _vp, _vp]),
     "onebit_unpack_to_dense": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp]),
     "onebit_check_device_status": (_int, []),
+    # the operators between the linear layers of a decoder block
+    "onebit_residual_norm": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _f32, _f32, _int, _vp]),
+    "onebit_rotary": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _vp, _int, _int, _f32, _i64, _i64, _i64, _int, _vp]),
+    "onebit_cache_append": (_int, [_vp, _i64, _i64] * 4 + [_vp, _int, _int, _f32] + [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] * 7 + [_int, _vp]),
+    "onebit_cache_attend_workspace": (_sz, [_i64] * 7),
+    "onebit_cache_attend": (_int, [_vp, _i64, _i64] * 2 + [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] * 8 + [_f32, _int, _int, _vp, _sz, _vp]),
 }
 # the reference's own entry point keeps its C++-mangled name
 LEGACY_SYMBOL = "_Z20onebit_sparse_matmulPvS_S_S_S_iii"

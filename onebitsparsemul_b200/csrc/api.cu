@@ -333,6 +333,119 @@ int onebit_unpack_to_dense(const void* bits_tile, const void* meta_tile, const v
   return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "unpack launch");
 }
 
+// ---- the operators between the linear layers of a decoder block ----------------------------------------------------------
+namespace {
+// codes below this one are bounded waits that gave up; see block_common.h
+constexpr int kStatusBadBatch = 64;
+
+int check_type(int dtype) {
+  return dtype == OB_DENSE_F16 || dtype == OB_DENSE_BF16 ? ONEBIT_OK : fail(ONEBIT_ERR_ARG, "unknown 16-bit type %d", dtype);
+}
+int check_rotation(const double* inv_freq, int rotary_dim, int64_t head_dim) {
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    return fail(ONEBIT_ERR_SHAPE, "rotary_dim = %d must be even and at most head_dim = %lld", rotary_dim, (long long)head_dim);
+  return rotary_dim > 0 && !inv_freq ? fail(ONEBIT_ERR_NULL, "null frequencies") : ONEBIT_OK;
+}
+int check_batch(const void* q_start, const void* kv_len, const void* table, int64_t table_width, int64_t tokens, int64_t seqs,
+                int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pages) {
+  if (!q_start || !kv_len || !table) return fail(ONEBIT_ERR_NULL, "null batch pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(ONEBIT_ERR_SHAPE, "the cache takes heads of 64 or 128 values (got %lld)", (long long)head_dim);
+  if (kv_heads < 1 || kv_heads > 4096 || heads < 1 || heads > 4096 || heads % kv_heads != 0)
+    return fail(ONEBIT_ERR_SHAPE, "heads = %lld must be a multiple of kv_heads = %lld, both from 1 to 4096", (long long)heads, (long long)kv_heads);
+  if (tokens < 0 || tokens > (1 << 24) || seqs < 1 || seqs > (1 << 16) || pages < 1 || pages > (1ll << 31) - 1 || table_width < 1 || table_width > (1 << 24))
+    return fail(ONEBIT_ERR_SHAPE, "tokens, sequences, pages or block table outside the supported range");
+  return ONEBIT_OK;
+}
+}  // namespace
+
+int onebit_residual_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int residual_f32, const void* gate,
+                         int64_t gate_stride, const void* post_weight, const void* weight, void* y, int64_t y_stride, void* h,
+                         int64_t h_stride, int64_t rows, int64_t hidden, float residual_scale, float eps, int dtype, void* stream) {
+  if (!x || !weight || !y || (residual && !h)) return fail(ONEBIT_ERR_NULL, "null operand pointer");
+  if (!residual && (gate || post_weight)) return fail(ONEBIT_ERR_ARG, "gate and post_weight need a residual");
+  if (int rc = check_type(dtype)) return rc;
+  if (rows < 0 || rows > (1ll << 31) - 1 || hidden < 1 || hidden > ONEBIT_NORM_MAX_HIDDEN)
+    return fail(ONEBIT_ERR_SHAPE, "need 1 <= hidden <= %d and fewer than 2^31 rows (got %lld x %lld)", ONEBIT_NORM_MAX_HIDDEN, (long long)rows, (long long)hidden);
+  if (rows == 0) return ONEBIT_OK;
+  cudaError_t e = ob::launch_residual_norm(x, x_stride, residual, residual_stride, residual_f32 != 0, gate, gate_stride, post_weight, weight,
+                                           y, y_stride, h, h_stride, rows, hidden, residual_scale, eps, dtype == OB_DENSE_BF16,
+                                           static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "residual norm launch");
+}
+
+int onebit_rotary(const void* x, int64_t x_token_stride, int64_t x_head_stride, void* y, int64_t y_token_stride, int64_t y_head_stride,
+                  const void* positions, int positions_i64, const double* inv_freq, int rotary_dim, int interleaved, float magnitude,
+                  int64_t tokens, int64_t heads, int64_t head_dim, int dtype, void* stream) {
+  if (!x || !y || !positions) return fail(ONEBIT_ERR_NULL, "null operand pointer");
+  if (int rc = check_type(dtype)) return rc;
+  if (tokens < 0 || tokens > (1 << 24) || heads < 1 || heads > 4096 || head_dim < 1 || head_dim > ONEBIT_ROTARY_MAX_DIM)
+    return fail(ONEBIT_ERR_SHAPE, "tokens = %lld, heads = %lld or head_dim = %lld outside the supported range", (long long)tokens, (long long)heads, (long long)head_dim);
+  if (int rc = check_rotation(inv_freq, rotary_dim, head_dim)) return rc;
+  if (tokens == 0) return ONEBIT_OK;
+  cudaError_t e = ob::launch_rotary(x, x_token_stride, x_head_stride, y, y_token_stride, y_head_stride, positions, positions_i64 != 0, inv_freq,
+                                    rotary_dim, interleaved != 0, magnitude, tokens, heads, head_dim, dtype == OB_DENSE_BF16,
+                                    static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "rotary launch");
+}
+
+int onebit_cache_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                        const double* inv_freq, int rotary_dim, int interleaved, float magnitude, void* k_pages, void* v_pages,
+                        float* k_scale, float* v_scale, int64_t pages, const int* q_start, const int* kv_len, const int* block_table,
+                        int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                        int64_t head_dim, int dtype, void* stream) {
+  if (!k || !v || !k_pages || !v_pages || !k_scale || !v_scale || (q && !q_out)) return fail(ONEBIT_ERR_NULL, "null operand pointer");
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_batch(q_start, kv_len, block_table, table_width, tokens, seqs, q ? heads : kv_heads, kv_heads, head_dim, pages)) return rc;
+  if (int rc = check_rotation(inv_freq, rotary_dim, head_dim)) return rc;
+  if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) return fail(ONEBIT_ERR_ARG, "pages must be 16-byte aligned");
+  if (tokens == 0) return ONEBIT_OK;
+  ob::CacheAppendCall c{k, v, q, q_out, k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride,
+                        q_out_token_stride, q_out_head_stride, inv_freq, rotary_dim, interleaved != 0, magnitude, k_pages, v_pages, k_scale, v_scale,
+                        pages, q_start, kv_len, block_table, table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim, dtype == OB_DENSE_BF16};
+  cudaError_t e = ob::launch_cache_append(c, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "cache append launch");
+}
+
+namespace {
+ob::CacheAttendCall attend_shape(int64_t pages, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new) {
+  ob::CacheAttendCall c{};
+  c.pages = pages, c.table_width = table_width, c.tokens = tokens, c.seqs = seqs, c.heads = heads, c.kv_heads = kv_heads, c.head_dim = head_dim;
+  c.max_new = max_new > 0 && max_new < tokens ? max_new : tokens;
+  return c;
+}
+}  // namespace
+
+size_t onebit_cache_attend_workspace(int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || seqs < 1 || tokens < 1) return 0;
+  return (size_t)ob::cache_attend_workspace(attend_shape(1, table_width, tokens, seqs, heads, kv_heads, head_dim, max_new));
+}
+
+int onebit_cache_attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                        const void* k_pages, const void* v_pages, const float* k_scale, const float* v_scale, int64_t pages,
+                        const int* q_start, const int* kv_len, const int* block_table, int64_t table_stride, int64_t table_width,
+                        int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, float scale,
+                        int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !out || !k_pages || !v_pages || !k_scale || !v_scale) return fail(ONEBIT_ERR_NULL, "null operand pointer");
+  if (int rc = check_type(dtype)) return rc;
+  if (int rc = check_batch(q_start, kv_len, block_table, table_width, tokens, seqs, heads, kv_heads, head_dim, pages)) return rc;
+  if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) return fail(ONEBIT_ERR_ARG, "pages must be 16-byte aligned");
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || ((q_token_stride | q_head_stride | out_token_stride | out_head_stride) & 7))
+    return fail(ONEBIT_ERR_ARG, "q and out must be 16-byte aligned with strides that are multiples of 8");
+  if (tokens == 0) return ONEBIT_OK;
+  ob::CacheAttendCall c = attend_shape(pages, table_width, tokens, seqs, heads, kv_heads, head_dim, max_new);
+  c.q = q, c.out = out, c.q_ts = q_token_stride, c.q_hs = q_head_stride, c.o_ts = out_token_stride, c.o_hs = out_head_stride;
+  c.k_pages = k_pages, c.v_pages = v_pages, c.k_scale = k_scale, c.v_scale = v_scale;
+  c.q_start = q_start, c.kv_len = kv_len, c.table = block_table, c.table_stride = table_stride;
+  c.scale = scale, c.causal = causal != 0, c.bf16 = dtype == OB_DENSE_BF16;
+  const int64_t need = ob::cache_attend_workspace(c);
+  if (need > 0 && (!workspace || (int64_t)workspace_bytes < need))
+    return fail(ONEBIT_ERR_WORKSPACE, "workspace of %zu bytes given, %lld needed", workspace ? workspace_bytes : (size_t)0, (long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(ONEBIT_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  cudaError_t e = ob::launch_cache_attend(c, workspace, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "cache attention launch");
+}
+
 // Reads and clears the status words of the tensor-memory and decode kernels on the current device. Synchronises
 // the device. Returns ONEBIT_ERR_DEVICE_WAIT if a bounded wait inside a kernel gave up since the
 // last call.
@@ -354,6 +467,13 @@ int onebit_check_device_status(void) {
   e = ob::read_fewtok_status(&host);
   if (e != cudaSuccess) return cuda_fail(e, "read_fewtok_status");
   if (host != 0) return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the few-token kernel gave up (code %d)", host);
+  e = ob::read_append_status(&host);
+  if (e != cudaSuccess) return cuda_fail(e, "read_append_status");
+  if (host != 0) return fail(ONEBIT_ERR_BATCH, "cache append: a page number or a sequence offset is outside its range (that page was not written)");
+  e = ob::read_attend_status(&host);
+  if (e != cudaSuccess) return cuda_fail(e, "read_attend_status");
+  if (host >= kStatusBadBatch) return fail(ONEBIT_ERR_BATCH, "cache attention: a page number or a sequence offset is outside its range (those tokens were left out)");
+  if (host != 0) return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the cache attention kernel gave up (code %d)", host);
   return ONEBIT_OK;
 }
 

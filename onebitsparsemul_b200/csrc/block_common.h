@@ -1,0 +1,97 @@
+// Shared pieces of the decoder-block kernels (norm.cu, rotary_append.cu, cache_attend*.cu). Internal header.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ob_block {
+
+// A cache page holds 64 tokens: keys (page, head, 64, dim), values (page, head, dim, 64), both e4m3, one fp32 scale for
+// each page and head of either.
+constexpr int kPageTokens = 64;
+constexpr float kE4m3Max = 448.f;
+constexpr int kMinScaleExp = -32, kMaxScaleExp = 32;
+
+// codes of the block kernels' status words
+constexpr int kStatusBadBatch = 64;   // a page number or a sequence offset outside its range: that work was skipped
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 8 consecutive values, 16-byte aligned for the 16-bit types and 32-byte for fp32
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(ws[i], T{});
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{}), pack2(v[4], v[5], T{}), pack2(v[6], v[7], T{}));
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// ---- rotary angles -----------------------------------------------------------------------------------------------------
+// An angle is kept in turns, as a 64-bit binary fraction: the frequency's share of a turn per position, rounded to 2^-64
+// (from a double: 53 bits of it are meaningful), times the position, modulo 2^64 -- the integer product wraps exactly where
+// the angle does. A position p adds an error of at most p * 2^-54 of a turn, so far positions cost nothing, where an fp32
+// product p * freq is off by p * 2^-24 radians.
+__device__ __forceinline__ uint64_t turns_per_position(double angular_frequency) {
+  double t = angular_frequency * 0.15915494309189533577;   // 1 / (2 pi)
+  t -= floor(t);
+  return __double2ull_rz(t * 18446744073709551616.0);
+}
+__device__ __forceinline__ float2 cos_sin(uint64_t per_position, int64_t position, float magnitude) {
+  const uint64_t phase = per_position * (uint64_t)position;
+  float s, c;
+  sincospif((float)(int32_t)(uint32_t)(phase >> 32) * 4.656612873077393e-10f /* 2^-31: half turns in [-1, 1) */, &s, &c);
+  return make_float2(c * magnitude, s * magnitude);
+}
+
+// ---- e4m3 -----------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float from_e4m3(uint8_t c) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+  return __half2float(__half(h));
+}
+// The smallest power of two 2^e, e in [-32, 32], with amax <= 448 * 2^e. A power of two keeps every division by the scale
+// exact, and a page that is re-scaled later only loses bits that leave e4m3's range.
+__device__ __forceinline__ float scale_for(float amax) {
+  if (!(amax > 0.f)) return exp2f((float)kMinScaleExp);
+  int e;
+  const float m = frexpf(amax, &e);                         // amax = m * 2^e, m in [0.5, 1); 448 = 0.875 * 2^9
+  e = m <= 0.875f ? e - 9 : e - 8;
+  return ldexpf(1.f, min(max(e, kMinScaleExp), kMaxScaleExp));
+}
+
+}  // namespace ob_block

@@ -59,4 +59,49 @@ cudaError_t launch_gemm_fewtok(const void* bits_tile, const void* meta_tile, con
                                bool fresh_weights, cudaStream_t stream);
 cudaError_t read_fewtok_status(int* out);
 
+// ---- the operators between the linear layers of a decoder block ----
+// residual add and norms (norm.cu); strides in elements from row to row, gate_stride 0 = one gate row for all rows
+cudaError_t launch_residual_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, bool residual_f32,
+                                 const void* gate, int64_t gate_stride, const void* post_weight, const void* weight, void* y,
+                                 int64_t y_stride, void* h, int64_t h_stride, int64_t rows, int64_t hidden, float residual_scale,
+                                 float eps, bool bf16, cudaStream_t stream);
+// rotary positions and cache append (rotary_append.cu); _ts / _hs: elements from one token / head to the next
+cudaError_t launch_rotary(const void* x, int64_t x_ts, int64_t x_hs, void* y, int64_t y_ts, int64_t y_hs, const void* positions,
+                          bool positions_i64, const double* inv_freq, int rotary_dim, bool interleaved, float magnitude, int64_t tokens,
+                          int64_t heads, int64_t head_dim, bool bf16, cudaStream_t stream);
+struct CacheAppendCall {
+  const void *k, *v, *q;
+  void* q_out;
+  int64_t k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, qo_ts, qo_hs;
+  const double* inv_freq;
+  int rotary_dim;              // 0: nothing is turned
+  bool interleaved;
+  float magnitude;
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  int64_t pages;
+  const int *q_start, *kv_len, *table;
+  int64_t table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim;
+  bool bf16;
+};
+cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream);
+cudaError_t read_append_status(int* out);
+// attention over the cache (cache_attend.cu)
+struct CacheAttendCall {
+  const void* q;
+  void* out;
+  int64_t q_ts, q_hs, o_ts, o_hs;
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  int64_t pages;
+  const int *q_start, *kv_len, *table;
+  int64_t table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim;
+  int64_t max_new;             // the caller's bound of a sequence's new tokens: it picks the kernel, no result depends on it
+  float scale;
+  bool causal, bf16;
+};
+int64_t cache_attend_workspace(const CacheAttendCall& c);
+cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream);
+cudaError_t read_attend_status(int* out);
+
 }  // namespace ob

@@ -1,0 +1,166 @@
+// Residual add with the norms around it, one pass over the row:
+//   u = x                                                        (no post_weight)
+//   u = x / sqrt(mean(x^2) + eps) * post_weight                  (a norm after the block)
+//   h = residual + residual_scale * gate * u                     (gate: one value per channel, per value, or absent)
+//   y = h / sqrt(mean(h^2) + eps) * weight                       (the norm before the next block; of h before its rounding)
+// Without a residual h = x and only y is written. The row lives in registers between its one read and its one write, both
+// sums are fp32: per-thread partial sums, then shuffles (and, above one warp per row, shared memory) in a fixed order.
+#include "block_common.h"
+#include "kernels.h"
+
+namespace {
+
+using namespace ob_block;
+
+struct NormArgs {
+  const void *x, *residual, *gate, *post_weight, *weight;
+  void *y, *h;
+  int64_t x_stride, r_stride, g_stride, y_stride, h_stride;   // elements from one row to the next; g_stride 0: one gate row for all
+  int64_t rows;
+  int hidden;
+  float residual_scale, eps;
+};
+
+// sum over the threads of one row
+template <bool WARP_ROW> __device__ __forceinline__ float row_sum(float v, float* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if (WARP_ROW) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  v = lane < warps ? scratch[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// V chunks of W values per thread; chunk j of thread t starts at value (j * threads_of_row + t) * W. W = 8: 16-byte accesses
+// (hidden % 8 == 0 and every row aligned); W = 1: any width and alignment.
+template <typename T, typename R, int V, int W, bool WARP_ROW>
+__global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a) {
+  __shared__ float scratch[2][32];
+  const int tpr = WARP_ROW ? 32 : blockDim.x;
+  const int t = WARP_ROW ? (threadIdx.x & 31) : threadIdx.x;
+  const int64_t row = WARP_ROW ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows) return;                                  // whole warps (WARP_ROW); never otherwise
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const R* res = a.residual ? static_cast<const R*>(a.residual) + row * a.r_stride : nullptr;
+  const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.g_stride : nullptr;
+  const T* post = static_cast<const T*>(a.post_weight);
+  const T* weight = static_cast<const T*>(a.weight);
+  T* y = static_cast<T*>(a.y) + row * a.y_stride;
+  R* hout = res ? static_cast<R*>(a.h) + row * a.h_stride : nullptr;
+  const float inv_n = 1.f / (float)a.hidden;
+
+  float u[V][W], r[V][W];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = (j * tpr + t) * W;
+    const bool in = c < a.hidden;
+    if constexpr (W == 8) {
+      if (in) { load8(x + c, u[j]); if (res) load8(res + c, r[j]); }
+      else for (int i = 0; i < W; ++i) u[j][i] = r[j][i] = 0.f;
+    } else {
+      u[j][0] = in ? to_f32(x[c]) : 0.f;
+      r[j][0] = in && res ? to_f32(res[c]) : 0.f;
+    }
+  }
+  if (res) {
+    float f = 1.f;
+    if (post) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < W; ++i) s += u[j][i] * u[j][i];
+      f = rsqrtf(row_sum<WARP_ROW>(s, scratch[0]) * inv_n + a.eps);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (j * tpr + t) * W;
+      if (c >= a.hidden) continue;
+      float p[W], g[W];
+      if constexpr (W == 8) {
+        if (post) load8(post + c, p);
+        if (gate) load8(gate + c, g);
+      } else {
+        if (post) p[0] = to_f32(post[c]);
+        if (gate) g[0] = to_f32(gate[c]);
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        float v = u[j][i];
+        if (post) v *= f * p[i];
+        if (gate) v *= g[i];
+        u[j][i] = r[j][i] + a.residual_scale * v;
+      }
+      if constexpr (W == 8) store8(hout + c, u[j]);
+      else hout[c] = from_f32<R>(u[j][0]);
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += u[j][i] * u[j][i];
+  const float f = rsqrtf(row_sum<WARP_ROW>(s, scratch[1]) * inv_n + a.eps);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = (j * tpr + t) * W;
+    if (c >= a.hidden) continue;
+    if constexpr (W == 8) {
+      float w[8];
+      load8(weight + c, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] *= u[j][i] * f;
+      store8(y + c, w);
+    } else {
+      y[c] = from_f32<T>(u[j][0] * f * to_f32(weight[c]));
+    }
+  }
+}
+
+template <typename T, typename R, int V, int W>
+cudaError_t launch_rows(const NormArgs& a, int threads, cudaStream_t stream) {
+  if (threads == 32) {
+    constexpr int kRows = 4;                                  // rows (warps) per CTA
+    ob_residual_norm_kernel<T, R, V, W, true><<<(unsigned)((a.rows + kRows - 1) / kRows), 32 * kRows, 0, stream>>>(a);
+  } else {
+    ob_residual_norm_kernel<T, R, V, W, false><<<(unsigned)a.rows, threads, 0, stream>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T, typename R> cudaError_t launch_types(const NormArgs& a, bool wide, cudaStream_t stream) {
+  const int chunks = wide ? a.hidden / 8 : a.hidden;
+  auto threads_for = [&](int per) { return max(32, min(1024, ((chunks + per - 1) / per + 31) / 32 * 32)); };
+  if (wide) {
+    if (chunks <= 1024) return launch_rows<T, R, 2, 8>(a, threads_for(2), stream);
+    return launch_rows<T, R, 4, 8>(a, threads_for(4), stream);
+  }
+  if (chunks <= 4096) return launch_rows<T, R, 8, 1>(a, threads_for(8), stream);
+  return launch_rows<T, R, 32, 1>(a, threads_for(32), stream);
+}
+
+}  // namespace
+
+namespace ob {
+
+cudaError_t launch_residual_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, bool residual_f32,
+                                 const void* gate, int64_t gate_stride, const void* post_weight, const void* weight, void* y,
+                                 int64_t y_stride, void* h, int64_t h_stride, int64_t rows, int64_t hidden, float residual_scale,
+                                 float eps, bool bf16, cudaStream_t stream) {
+  const NormArgs a{x, residual, gate, post_weight, weight, y, h, x_stride, residual_stride, gate_stride, y_stride, h_stride,
+                   rows, (int)hidden, residual_scale, eps};
+  auto rows_ok = [](const void* p, int64_t stride) {   // every row starts on a 16-byte boundary
+    return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0);
+  };
+  const bool wide = hidden % 8 == 0 && rows_ok(x, x_stride) && rows_ok(residual, residual_stride) &&
+                    rows_ok(gate, gate_stride) && rows_ok(post_weight, 0) && rows_ok(weight, 0) && rows_ok(y, y_stride) &&
+                    rows_ok(h, h_stride);
+  if (bf16) return residual_f32 ? launch_types<__nv_bfloat16, float>(a, wide, stream) : launch_types<__nv_bfloat16, __nv_bfloat16>(a, wide, stream);
+  return residual_f32 ? launch_types<__half, float>(a, wide, stream) : launch_types<__half, __half>(a, wide, stream);
+}
+
+}  // namespace ob

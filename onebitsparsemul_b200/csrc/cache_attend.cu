@@ -1,95 +1,575 @@
-// Attention over the 8-bit cache, plain form: one warp per query row.
+// Attention over the 8-bit cache for few query rows per cache head (decode steps, drafted tokens).
+//
+// out = softmax(scale q K^T) V; the work is to stream every cached byte once. For at most 16 query rows the products are
+// padding on the tensor cores whatever is done, so the kernel is built around the stream:
+//   * the pages of all (sequence, cache head, row tile) segments form one line that is cut into equal pieces, one per CTA, two
+//     CTAs per SM: a ragged batch is balanced without the host knowing a length. A segment that a cut falls into leaves
+//     partial results, which a second small kernel joins (ob_attend_combine_kernel);
+//   * every warp takes every fourth page of its CTA's piece and fetches it by itself: bulk asynchronous copies (keys, then
+//     values: 64 * D bytes each, contiguous) into a ring of its own, so no warp ever waits for another inside a segment;
+//   * keys are the A operand of S^T = K Q^T (16 tokens x 16 values, mma m16n8k16, N = 8 query rows), values of O^T = V^T P^T:
+//     the query rows are the narrow dimension, so 8 rows cost half of what they would as 16 padded ones. The order of the
+//     contraction is free, so a thread's operands are 16 consecutive bytes: four k-steps of a key row, or of a value row's
+//     tokens; the token that stands in row i of a score tile is chosen so that both fit. P goes from the accumulator layout to
+//     the B operand by movmatrix (8 x 8 transposes);
+//   * e4m3 -> fp16 is exact; the page's key scale multiplies the fp32 scores. The value scale goes
+//     into the exponent: t = score + log2(value scale), running maximum M of t, weight w = 2^(t - M) rounded to fp16 (2^-11, the
+//     only rounding before the output's), and the sum of the weights without it is sum(w / value scale), in fp32.
+// bf16 queries become fp16 with a power of two per row (the row's largest value lands in [1, 2)): their 8 bits fit; a value
+// 2^-14 below the row's largest starts losing bits of no consequence.
+#include <algorithm>
+#include <type_traits>
+
 #include "block_common.h"
 #include "kernels.h"
+#include "sm100_ptx.h"
 
 namespace {
 
 using namespace ob_block;
+using namespace ob_ptx;
 
 __device__ int g_attend_status;
 
-template <typename T, int D> __global__ void __launch_bounds__(128) ob_cache_attend_simple_kernel(const ob::CacheAttendCall c) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + warp;
-  if (row >= c.tokens * c.heads) return;
-  const int t = (int)(row / c.heads), head = (int)(row % c.heads);
-  int count = 0;
-  for (int s0 = 0; s0 <= c.seqs; s0 += 32) count += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && c.q_start[s0 + lane] <= t));
-  if (count < 1 || count > c.seqs) return;
-  const int seq = count - 1;
-  const int kv = min(c.kv_len[seq], (int)c.table_width * kPageTokens);
-  const int limit = c.causal ? min(kv, c.kv_len[seq] - c.q_start[seq + 1] + t + 1) : kv;   // tokens that this row sees
-  const int kvh = head / (int)(c.heads / c.kv_heads);
-  __shared__ float qs[4][D];
-  const T* q = static_cast<const T*>(c.q) + t * c.q_ts + head * c.q_hs;
-  for (int d = lane; d < D; d += 32) qs[warp][d] = to_f32(q[d]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, o[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-  for (int p0 = 0; p0 < limit; p0 += kPageTokens) {
-    const int page = c.table[seq * c.table_stride + p0 / kPageTokens];
-    if (page < 0 || page >= c.pages) {
-      if (lane == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
-      continue;
-    }
-    const int64_t ph = (int64_t)page * c.kv_heads + kvh;
-    const uint8_t* kp = static_cast<const uint8_t*>(c.k_pages) + ph * kPageTokens * D;
-    const uint8_t* vp = static_cast<const uint8_t*>(c.v_pages) + ph * kPageTokens * D;
-    const float ks = c.k_scale[ph] * c.scale, vs = c.v_scale[ph];
-    float s[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int tok = lane + 32 * h;
-      float acc = 0.f;
-      for (int d = 0; d < D; ++d) acc += qs[warp][d] * from_e4m3(kp[tok * D + d]);
-      s[h] = p0 + tok < limit ? acc * ks : -INFINITY;
-    }
-    float mx = fmaxf(s[0], s[1]);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, k));
-    const float mn = fmaxf(m, mx);
-    const float f = m == -INFINITY ? 0.f : __expf(m - mn);
-    l *= f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] *= f;
-    m = mn;
-    float pr[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      pr[h] = p0 + lane + 32 * h < limit ? expf(s[h] - mn) : 0.f;
-      l += pr[h];
-    }
-    const int seen = min(kPageTokens, limit - p0);
-    for (int tok = 0; tok < seen; ++tok) {
-      const float w = __shfl_sync(~0u, tok < 32 ? pr[0] : pr[1], tok & 31) * vs;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] += w * from_e4m3(vp[(lane + 32 * i) * kPageTokens + tok]);
-    }
+constexpr int kWarps = 4;
+constexpr int kRingBytes = 24 * 1024;             // per warp
+constexpr int kMinPages = 4;                      // pages of a CTA's piece: one per warp
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- the line of pages ------------------------------------------------------------------------------------------------
+
+struct Seq {
+  int q0, n, kv, pages, tiles;                    // kv: cached tokens; pages: 0 if the sequence has no new token, else at least 1
+  int64_t w;                                      // pages of all its segments
+};
+
+__device__ __forceinline__ Seq seq_info(const ob::CacheAttendCall& c, int s, int rows_per_tile) {
+  Seq q;
+  const int q1 = __ldg(c.q_start + s + 1);
+  q.q0 = __ldg(c.q_start + s);
+  q.kv = __ldg(c.kv_len + s);
+  q.n = q.q0 < 0 || q1 > c.tokens || q1 < q.q0 ? 0 : q1 - q.q0;
+  const int64_t room = c.table_width * kPageTokens;
+  const int seen = (int)min((int64_t)max(q.kv, 0), room);
+  q.pages = q.n > 0 ? max(1, (seen + kPageTokens - 1) / kPageTokens) : 0;
+  q.tiles = (int)((q.n * (c.heads / c.kv_heads) + rows_per_tile - 1) / rows_per_tile);
+  q.w = (int64_t)q.pages * q.tiles * c.kv_heads;
+  return q;
+}
+
+// What a combine block needs of the segment that starts in CTA c and ends in CTA last (-1: there is none).
+struct alignas(16) Header {
+  int last, q0, n, head, tile, pad[3];
+};
+
+struct FewLayout {                                // the workspace
+  Header* headers;
+  float* partial;                                 // slots 2 c (segment that started before CTA c), 2 c + 1: rows x (D + 4): M, l at [D], [D + 1]
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// two e4m3 bytes (low or high half of a word) -> two fp16
+__device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// NT tiles of 8 query rows
+template <typename T, int D, int NT> __global__ void __launch_bounds__(kWarps * 32, 2)
+ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
+  constexpr int kRows = 8 * NT;
+  constexpr int kGranule = kPageTokens * D;                     // bytes of one page's keys (or values) of a head
+  constexpr int kRing = kRingBytes / kGranule;
+  constexpr int kMeta = 4;                                      // pages between a request and its use, at most kRing / 2 + 1
+  constexpr int kMT = D / 16;                                   // value tiles
+  constexpr int kPitch = D + 4;
+  static_assert(kRing / 2 + 1 <= kMeta, "page data ring");
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* merge = reinterpret_cast<float*>(smem + kWarps * kRingBytes);           // [warp][8][kPitch]
+  struct Meta { float ks, log2_vs, inv_vs; int ok; };
+  __shared__ Meta meta[kWarps][kMeta];
+  __shared__ __align__(8) uint64_t bars[kWarps][kRing];
+  __shared__ int64_t scan[kWarps + 1];
+  __shared__ int64_t start_off;
+  __shared__ int start_seq;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = (int)(c.heads / c.kv_heads);
+  const int H = (int)c.kv_heads;
+  long long budget = 2000000000ll;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (lane == 0)
+    for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+
+  // ---- this CTA's piece: every thread sums a run of sequences, the CTA scans the sums ----
+  const int run = (int)((c.seqs + kWarps * 32 - 1) / (kWarps * 32));
+  const int s_lo = min((int)c.seqs, (int)threadIdx.x * run), s_hi = min((int)c.seqs, s_lo + run);
+  int64_t mine = 0;
+  bool bad = false;
+  for (int s = s_lo; s < s_hi; ++s) {
+    const Seq q = seq_info(c, s, kRows);
+    mine += q.w;
+    bad |= q.n == 0 && (__ldg(c.q_start + s) < 0 || __ldg(c.q_start + s + 1) > c.tokens);
   }
+  if (bad && blockIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+  int64_t upto = mine;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) l += __shfl_xor_sync(~0u, l, k);
-  T* out = static_cast<T*>(c.out) + t * c.o_ts + head * c.o_hs;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(~0u, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  int64_t W = 0, before_warp = 0;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp) before_warp = W;
+    W += scan[w];
+  }
+  upto += before_warp;                                          // pages of the sequences up to this thread's last
+  const int64_t chunk = max((int64_t)kMinPages, (W + gridDim.x - 1) / gridDim.x);
+  const int64_t a = blockIdx.x * chunk, b = min(a + chunk, W);
+  if (a >= W) {
+    if (threadIdx.x == 0) ws.headers[blockIdx.x].last = -1;
+    return;
+  }
+  if (a >= upto - mine && a < upto) {
+    int64_t off = a - (upto - mine);
+    int s = s_lo;
+    for (Seq q = seq_info(c, s, kRows); off >= q.w; q = seq_info(c, s, kRows)) { off -= q.w; ++s; }
+    start_seq = s;
+    start_off = off;
+  }
+  __syncthreads();
+  int seq = start_seq;
+  int64_t off = start_off;
+
+  // ---- requests: this warp's pages are those at a + warp, a + warp + 4, ...; 32 of them are looked up at a time, one per lane ----
+  const int my_pages = (int)max((int64_t)0, (b - a - warp + kWarps - 1) / kWarps);
+  int load_seq = seq;
+  int64_t load_off = off + warp;
+  int64_t ph = -1;                                              // (page, head) of this lane's page; -1: nothing to fetch
+  float ph_ks = 0.f, ph_lvs = 0.f, ph_ivs = 1.f;
+  const uint32_t ring = smem_u32(smem) + warp * kRingBytes;
+  auto look_up = [&](int first) {                               // pages first .. first + 31
+    int s = load_seq;
+    int64_t o = load_off + (int64_t)lane * kWarps;
+    ph = -1;
+    if (first + lane < my_pages) {
+      Seq q = seq_info(c, s, kRows);
+      while (o >= q.w) { o -= q.w; q = seq_info(c, ++s, kRows); }
+      const int64_t seg = o / q.pages;
+      const int pg = (int)(o - seg * q.pages), head = (int)(seg / q.tiles);
+      if ((int64_t)pg * kPageTokens < q.kv) {
+        const int id = __ldg(c.table + (int64_t)s * c.table_stride + pg);
+        if (id < 0 || id >= c.pages) {
+          atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+        } else {
+          ph = (int64_t)id * H + head;
+          ph_ks = __ldg(c.k_scale + ph);
+          const float vs = fmaxf(__ldg(c.v_scale + ph), 5.421010862e-20f);   // 2^-64: a page that nothing was stored in has scale 0
+          ph_lvs = log2f(vs);
+          ph_ivs = 1.f / vs;
+        }
+      }
+    }
+    load_seq = __shfl_sync(~0u, s, 31);                         // where the next 32 begin, if there are any
+    load_off = __shfl_sync(~0u, o, 31) + kWarps;
+  };
+  // granule gr: keys (even) or values (odd) of page gr / 2, into slot gr % kRing
+  auto request = [&](int gr) {
+    const int i = gr >> 1;
+    if (i >= my_pages) return;
+    if ((i & 31) == 0 && (gr & 1) == 0) look_up(i);
+    const int64_t at = __shfl_sync(~0u, ph, i & 31);
+    const uint32_t bar = smem_u32(&bars[warp][gr % kRing]);
+    if ((gr & 1) == 0) {
+      if (lane == (i & 31)) meta[warp][i % kMeta] = {ph_ks, ph_lvs, ph_ivs, at >= 0};
+    }
+    if (lane == 0) {
+      if (at >= 0) {
+        mbar_expect_tx(bar, kGranule);
+        bulk_load(ring + (gr % kRing) * kGranule, static_cast<const uint8_t*>(gr & 1 ? c.v_pages : c.k_pages) + at * kGranule, kGranule, bar);
+      } else {
+        mbar_arrive(bar);
+      }
+    }
+  };
+  for (int gr = 0; gr < kRing; ++gr) request(gr);
+  __syncwarp();
+
+  int gr = 0;                                                   // granules used so far by this warp
+  for (int64_t l = a; l < b;) {
+    // ---- one segment's part in this piece ----
+    Seq q = seq_info(c, seq, kRows);
+    while (off >= q.w) { off -= q.w; q = seq_info(c, ++seq, kRows); }
+    const int64_t seg = off / q.pages;
+    const int page0 = (int)(off - seg * q.pages);
+    const int head = (int)(seg / q.tiles), tile = (int)(seg - (int64_t)head * q.tiles);
+    const int take = (int)min(b - l, (int64_t)(q.pages - page0));
+    const int rows_all = q.n * group;
+    const int kv = (int)min((int64_t)max(q.kv, 0), c.table_width * kPageTokens);
+
+    // queries: B operand of row g, and what the accumulators' columns 2 t, 2 t + 1 need
+    uint32_t qf[NT][D / 16][2];
+    float coef[NT][2];
+    int limit[NT][2], least = 0x7fffffff;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = tile * kRows + nt * 8 + g;
+      const bool in = r < rows_all;
+      const T* row = static_cast<const T*>(c.q) + (int64_t)(q.q0 + r / group) * c.q_ts + (int64_t)(head * group + r % group) * c.q_hs;
+      uint2 raw[D / 16];
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) raw[k] = in ? *reinterpret_cast<const uint2*>(row + (k / 4) * 64 + t * 16 + (k % 4) * 4) : make_uint2(0, 0);
+      float unit = 1.f;                                         // what the fp16 form is to be multiplied by
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const float2 x = unpack2(raw[k].x, T{}), y = unpack2(raw[k].y, T{});
+          m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+        }
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+        // the row's exponent, kept where both 2^e and 2^-e are normal numbers; an infinite row stays infinite
+        const int e = min(max((int)(__float_as_uint(m) >> 23), 2), 252);
+        unit = __uint_as_float((uint32_t)e << 23);
+        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const float2 x = unpack2(raw[k].x, T{}), y = unpack2(raw[k].y, T{});
+          raw[k] = make_uint2(pack2(x.x * inv, x.y * inv, __half{}), pack2(y.x * inv, y.y * inv, __half{}));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) { qf[nt][k][0] = raw[k].x; qf[nt][k][1] = raw[k].y; }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        coef[nt][j] = __shfl_sync(~0u, unit, (2 * t + j) * 4) * (c.scale * kLog2e);
+        const int rr = tile * kRows + nt * 8 + 2 * t + j;       // rows behind the last one see everything: nothing of theirs is kept
+        limit[nt][j] = rr >= rows_all ? 0x7fffffff : (c.causal ? min(kv, q.kv - q.n + rr / group + 1) : kv);
+        least = min(least, limit[nt][j]);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) least = min(least, __shfl_xor_sync(~0u, least, o));
+
+    float acc[NT][kMT][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) { m_run[nt][j] = -INFINITY; l_run[nt][j] = 0.f; }
+    }
+
+    for (int j = (int)((warp - (l - a)) & (kWarps - 1)); j < take; j += kWarps) {
+      const int base = (page0 + j) * kPageTokens;
+      const Meta md = meta[warp][(gr >> 1) % kMeta];
+      const int k_slot = gr % kRing, v_slot = (gr + 1) % kRing;
+      const uint32_t k_par = (gr / kRing) & 1, v_par = ((gr + 1) / kRing) & 1;
+      const uint8_t* kp = smem + warp * kRingBytes + k_slot * kGranule;
+      const uint8_t* vp = smem + warp * kRingBytes + v_slot * kGranule;
+      mbar_wait(smem_u32(&bars[warp][k_slot]), k_par, budget, &g_attend_status, 1);
+      __syncwarp();
+      float sc[NT][4][4];
+      if (md.ok) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {                           // 16 tokens: (g / 2) 16 + 4 s + (g odd), and 2 further
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[nt][s][i] = 0.f;
+          const uint8_t* k0 = kp + ((g >> 1) * 16 + 4 * s + (g & 1)) * D + t * 16;
+#pragma unroll
+          for (int hf = 0; hf < D / 64; ++hf) {
+            const uint4 x = *reinterpret_cast<const uint4*>(k0 + hf * 64), y = *reinterpret_cast<const uint4*>(k0 + 2 * D + hf * 64);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t a0 = e4m3_lo(xs[w]), a2 = e4m3_hi(xs[w]), a1 = e4m3_lo(ys[w]), a3 = e4m3_hi(ys[w]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_16816(sc[nt][s], a0, a1, a2, a3, qf[nt][hf * 4 + w][0], qf[nt][hf * 4 + w][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      request(gr + kRing);                                      // the keys' slot is free
+      uint32_t pf[NT][4][2];                                    // weights: B operand of k-step s
+      if (md.ok) {
+        bool moved = false;
+        float alpha[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float k0 = coef[nt][0] * md.ks, k1 = coef[nt][1] * md.ks;
+          float m0 = m_run[nt][0], m1 = m_run[nt][1];
+          const bool masked = base + kPageTokens > least;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x = fmaf(sc[nt][s][2 * h], k0, md.log2_vs), y = fmaf(sc[nt][s][2 * h + 1], k1, md.log2_vs);
+              if (masked) {
+                const int tok = base + (g >> 1) * 16 + 4 * s + 2 * h + (g & 1);
+                if (tok >= limit[nt][0]) x = -INFINITY;
+                if (tok >= limit[nt][1]) y = -INFINITY;
+              }
+              sc[nt][s][2 * h] = x;
+              sc[nt][s][2 * h + 1] = y;
+              m0 = fmaxf(m0, x);
+              m1 = fmaxf(m1, y);
+            }
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(~0u, m0, o));
+            m1 = fmaxf(m1, __shfl_xor_sync(~0u, m1, o));
+          }
+          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+          moved |= m0 != m_run[nt][0] || m1 != m_run[nt][1];
+          alpha[nt][0] = fast_exp2(m_run[nt][0] - r0);
+          alpha[nt][1] = fast_exp2(m_run[nt][1] - r1);
+          m_run[nt][0] = m0;
+          m_run[nt][1] = m1;
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = fast_exp2(sc[nt][s][2 * h] - r0), y = fast_exp2(sc[nt][s][2 * h + 1] - r1);
+              s0 += x;
+              s1 += y;
+              pf[nt][s][h] = transpose_8x8(pack2(x, y, __half{}));
+            }
+          }
+          l_run[nt][0] = l_run[nt][0] * alpha[nt][0] + s0 * md.inv_vs;
+          l_run[nt][1] = l_run[nt][1] * alpha[nt][1] + s1 * md.inv_vs;
+        }
+        if (__any_sync(~0u, moved)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < kMT; ++i) {
+              acc[nt][i][0] *= alpha[nt][0], acc[nt][i][1] *= alpha[nt][1];
+              acc[nt][i][2] *= alpha[nt][0], acc[nt][i][3] *= alpha[nt][1];
+            }
+        }
+      }
+      mbar_wait(smem_u32(&bars[warp][v_slot]), v_par, budget, &g_attend_status, 2);
+      __syncwarp();
+      if (md.ok) {
+        // bytes behind the sequence's end may be anything, a NaN among them: they are read as zeros
+        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+        const bool tail = base + kPageTokens > kv;
+        if (tail) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int live = kv - base - (t * 16 + 4 * s);
+            keep[s] = live >= 4 ? ~0u : live <= 0 ? 0u : ~0u >> (8 * (4 - live));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+          const uint8_t* v0 = vp + (16 * i + g) * kPageTokens + t * 16;
+          const uint4 x = *reinterpret_cast<const uint4*>(v0), y = *reinterpret_cast<const uint4*>(v0 + 8 * kPageTokens);
+          uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          if (tail) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) { xs[s] &= keep[s]; ys[s] &= keep[s]; }
+          }
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const uint32_t a0 = e4m3_lo(xs[s]), a2 = e4m3_hi(xs[s]), a1 = e4m3_lo(ys[s]), a3 = e4m3_hi(ys[s]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][i], a0, a1, a2, a3, pf[nt][s][0], pf[nt][s][1]);
+          }
+        }
+      }
+      __syncwarp();
+      request(gr + 1 + kRing);
+      gr += 2;
+      __syncwarp();
+    }
+
+    // ---- the four warps' results of the segment, 8 rows at a time ----
+    const bool from_before = page0 > 0 && l == a, goes_on = page0 + take < q.pages;
+    float* slot = ws.partial + (int64_t)(2 * blockIdx.x + (from_before ? 0 : 1)) * kRows * kPitch;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float* mw = merge + warp * 8 * kPitch;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float s = l_run[nt][j];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(~0u, s, o);
+        if (g == 0) { mw[(2 * t + j) * kPitch + D] = m_run[nt][j]; mw[(2 * t + j) * kPitch + D + 1] = s; }
+      }
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) {
+        mw[(2 * t) * kPitch + 16 * i + g] = acc[nt][i][0];
+        mw[(2 * t + 1) * kPitch + 16 * i + g] = acc[nt][i][1];
+        mw[(2 * t) * kPitch + 16 * i + 8 + g] = acc[nt][i][2];
+        mw[(2 * t + 1) * kPitch + 16 * i + 8 + g] = acc[nt][i][3];
+      }
+      __syncthreads();
+      {
+        const int row = threadIdx.x >> 4, x = threadIdx.x & 15;
+        float f[kWarps], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) { f[w] = merge[(w * 8 + row) * kPitch + D]; M = fmaxf(M, f[w]); }
+        const float R = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) { f[w] = fast_exp2(f[w] - R); L += f[w] * merge[(w * 8 + row) * kPitch + D + 1]; }
+        const int r = tile * kRows + nt * 8 + row;
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += 64) {
+          const int d = d0 + x * 4;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(&merge[(w * 8 + row) * kPitch + d]);
+            o.x += f[w] * v.x, o.y += f[w] * v.y, o.z += f[w] * v.z, o.w += f[w] * v.w;
+          }
+          if (from_before || goes_on) {
+            *reinterpret_cast<float4*>(slot + (nt * 8 + row) * kPitch + d) = o;
+            if (x == 0 && d0 == 0) { slot[(nt * 8 + row) * kPitch + D] = M; slot[(nt * 8 + row) * kPitch + D + 1] = L; }
+          } else if (r < rows_all) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            T* out = static_cast<T*>(c.out) + (int64_t)(q.q0 + r / group) * c.o_ts + (int64_t)(head * group + r % group) * c.o_hs + d;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack2(o.x * inv, o.y * inv, T{}), pack2(o.z * inv, o.w * inv, T{}));
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0 && l + take == b) {                    // the piece's last segment: does it start here and go on?
+      Header h{};
+      h.last = !from_before && goes_on ? (int)((l - page0 + q.pages - 1) / chunk) : -1;
+      h.q0 = q.q0, h.n = q.n, h.head = head, h.tile = tile;
+      ws.headers[blockIdx.x] = h;
+    }
+    l += take;
+    off += take;
+  }
+}
+
+// Joins the partial results of the segment that starts in piece blockIdx.x: one CTA per query row, every warp a share of the
+// pieces, in a fixed order.
+template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_combine_kernel(const ob::CacheAttendCall c, const FewLayout ws, int rows) {
+  constexpr int kPitch = D + 4;
+  __shared__ float red[8], total[8], part[8][D];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Header h = ws.headers[blockIdx.x];
+  if (h.last < 0) return;
+  const int group = (int)(c.heads / c.kv_heads);
+  const int row = blockIdx.y, r = h.tile * rows + row;
+  if (r >= h.n * group) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = h.last - (int)blockIdx.x + 1;
+  auto slot = [&](int i) {                                      // i-th partial of the segment
+    return ws.partial + ((int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * rows + row) * kPitch;
+  };
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < count; i += 256) m = fmaxf(m, slot(i)[D]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+  const float R = m == -INFINITY ? 0.f : m;
+  constexpr int kPer = D / 32;
+  float o[kPer] = {}, l = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < count; i += 8) {
+    const float* p = slot(i);
+    const float f = fast_exp2(p[D] - R);
+    l += f * p[D + 1];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] += f * p[lane + 32 * e];
+  }
+  if (lane == 0) total[warp] = l;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) part[warp][lane + 32 * e] = o[e];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float sum = 0.f, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) { sum += part[w][threadIdx.x]; L += total[w]; }
+    T* out = static_cast<T*>(c.out) + (int64_t)(h.q0 + r / group) * c.o_ts + (int64_t)(h.head * group + r % group) * c.o_hs;
+    out[threadIdx.x] = from_f32<T>(L == 0.f ? 0.f : sum / L);
+  }
+}
+
+int few_tiles(const ob::CacheAttendCall& c) { return c.max_new * (c.heads / c.kv_heads) <= 8 ? 1 : 2; }
+// two CTAs per SM, but no more pieces than the block table could fill
+int few_grid(const ob::CacheAttendCall& c) {
+  const int64_t rows = 8 * few_tiles(c), group = c.heads / c.kv_heads;
+  const int64_t tiles = (c.tokens * group + rows - 1) / rows + c.seqs;          // at least the row tiles of all sequences
+  const int64_t most = (tiles * c.kv_heads * c.table_width + kMinPages - 1) / kMinPages;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(2 * ob::sm_count(), most));
+}
+
+template <typename T, int D, int NT> cudaError_t launch_few(const ob::CacheAttendCall& c, void* workspace, cudaStream_t stream) {
+  const int grid = few_grid(c);
+  constexpr int smem = kWarps * kRingBytes + kWarps * 8 * (D + 4) * 4;
+  FewLayout ws{static_cast<Header*>(workspace), reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((grid * sizeof(Header) + 255) & ~size_t(255)))};
+  cudaError_t e = cudaFuncSetAttribute(ob_attend_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  ob_attend_few_kernel<T, D, NT><<<grid, kWarps * 32, smem, stream>>>(c, ws);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 8 * NT), cfg.blockDim = dim3(256), cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, ob_attend_combine_kernel<T, D>, c, ws, 8 * NT);
 }
 
 }  // namespace
 
 namespace ob {
 
-int64_t cache_attend_workspace(const CacheAttendCall&) { return 0; }
+int64_t cache_attend_workspace(const CacheAttendCall& c) {
+  const int64_t grid = few_grid(c);
+  return ((grid * (int64_t)sizeof(Header) + 255) & ~255ll) + 2 * grid * 8 * few_tiles(c) * (c.head_dim + 4) * 4;
+}
 
-cudaError_t launch_cache_attend(const CacheAttendCall& c, void*, cudaStream_t stream) {
-  const unsigned grid = (unsigned)((c.tokens * c.heads + 3) / 4);
-  if (c.bf16) {
-    if (c.head_dim == 64) ob_cache_attend_simple_kernel<__nv_bfloat16, 64><<<grid, 128, 0, stream>>>(c);
-    else ob_cache_attend_simple_kernel<__nv_bfloat16, 128><<<grid, 128, 0, stream>>>(c);
-  } else {
-    if (c.head_dim == 64) ob_cache_attend_simple_kernel<__half, 64><<<grid, 128, 0, stream>>>(c);
-    else ob_cache_attend_simple_kernel<__half, 128><<<grid, 128, 0, stream>>>(c);
-  }
-  return cudaGetLastError();
+cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream) {
+  auto by_tiles = [&](auto t, auto d) {
+    return few_tiles(c) == 1 ? launch_few<decltype(t), decltype(d)::value, 1>(c, workspace, stream)
+                             : launch_few<decltype(t), decltype(d)::value, 2>(c, workspace, stream);
+  };
+  auto by_dim = [&](auto t) {
+    return c.head_dim == 64 ? by_tiles(t, std::integral_constant<int, 64>{}) : by_tiles(t, std::integral_constant<int, 128>{});
+  };
+  return c.bf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
 }
 
 cudaError_t read_attend_status(int* out) {

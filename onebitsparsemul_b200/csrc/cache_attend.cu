@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "block_common.h"
+#include "cache_attend.h"
 #include "kernels.h"
 #include "sm100_ptx.h"
 
@@ -74,17 +75,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-// two e4m3 bytes (low or high half of a word) -> two fp16
-__device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
   return r;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -525,6 +515,8 @@ template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_co
   }
 }
 
+// Which kernel: both are right for any batch.
+bool many_rows(const ob::CacheAttendCall& c) { return c.max_new * (c.heads / c.kv_heads) > 32; }
 int few_tiles(const ob::CacheAttendCall& c) { return c.max_new * (c.heads / c.kv_heads) <= 8 ? 1 : 2; }
 // two CTAs per SM, but no more pieces than the block table could fill
 int few_grid(const ob::CacheAttendCall& c) {
@@ -557,11 +549,13 @@ template <typename T, int D, int NT> cudaError_t launch_few(const ob::CacheAtten
 namespace ob {
 
 int64_t cache_attend_workspace(const CacheAttendCall& c) {
+  if (many_rows(c)) return cache_attend_many_workspace(c);
   const int64_t grid = few_grid(c);
   return ((grid * (int64_t)sizeof(Header) + 255) & ~255ll) + 2 * grid * 8 * few_tiles(c) * (c.head_dim + 4) * 4;
 }
 
 cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream) {
+  if (many_rows(c)) return launch_cache_attend_many(c, workspace, stream);
   auto by_tiles = [&](auto t, auto d) {
     return few_tiles(c) == 1 ? launch_few<decltype(t), decltype(d)::value, 1>(c, workspace, stream)
                              : launch_few<decltype(t), decltype(d)::value, 2>(c, workspace, stream);
@@ -574,7 +568,8 @@ cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaS
 
 cudaError_t read_attend_status(int* out) {
   cudaError_t e = cudaMemcpyFromSymbol(out, g_attend_status, sizeof(int));
-  if (e != cudaSuccess || *out == 0) return e;
+  if (e != cudaSuccess) return e;
+  if (*out == 0) return read_attend_many_status(out);
   const int zero = 0;
   return cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
 }

@@ -1,0 +1,542 @@
+// Attention over the 8-bit cache for many query rows (prompts, chunks of prompts), on tcgen05.
+//
+// One CTA owns 256 query rows of a cache head -- the rows of all heads of its group, token by token, so that a group shares
+// the keys -- as two tiles of 128, and walks over the cached tokens 128 at a time:
+//   * producers (4 warps) fetch two pages' keys and values with 16-byte loads one step ahead, widen e4m3 to fp16 (exact) and
+//     store them as K-major operands with the 128-byte swizzle. The pages' layout makes both K-major: keys (token, dim) for
+//     S = Q K^T, values (dim, token) for O += P V. Widening once per CTA costs what a TMA load of fp16 would cost in shared
+//     memory, and the cache is read at 8 bits;
+//   * one thread issues tcgen05.mma (M = 128, fp32 accumulators in tensor memory): S of one tile is computed while the other
+//     tile's softmax runs;
+//   * softmax (4 warps per tile, thread = row): the row's scores are read from tensor memory, the weights go back as fp16 over
+//     the scores' own columns and are the A operand of the second product. The running maximum is only raised, and O
+//     multiplied, when it would otherwise let a weight pass 2^8: the sums are fp32, so a lower reference costs nothing.
+// Scales as in cache_attend.cu: the key scale multiplies the score, the value scale goes into the exponent.
+// Long caches with too few row tiles to fill the chip are split along the cached tokens; the parts are joined by a second kernel.
+// Every mbarrier wait is bounded. No TMA.
+#include <algorithm>
+#include <type_traits>
+
+#include "block_common.h"
+#include "cache_attend.h"
+#include "kernels.h"
+#include "sm100_ptx.h"
+
+namespace {
+
+using namespace ob_block;
+using namespace ob_ptx;
+
+__device__ int g_attend_many_status;
+
+constexpr int kTileRows = 128, kCtaRows = 256, kTileTokens = 128;
+constexpr int kProducers = 4;                                   // warps
+constexpr int kThreads = 32 * (8 + 1 + kProducers);
+constexpr float kRaise = 8.f;                                   // log2 of the largest weight before the reference is raised
+
+template <int D> struct Cfg {
+  static constexpr int kQBytes = kTileRows * D * 2;             // per tile
+  static constexpr int kKBytes = kTileTokens * D * 2, kVBytes = kKBytes;
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kSmem = 2 * kQBytes + kStages * (kKBytes + kVBytes) + 1024;
+  static_assert(kSmem <= 226 * 1024, "shared memory");
+  static constexpr int kTmemS = 0, kTmemO = 256;                // S / P of tile g at 128 g, O of tile g at 256 + D g
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1)
+ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  struct Meta { float ks, log2_vs, inv_vs, pad; };
+  // the pages of step j in [j % kMeta]: a stage is filled again when its scores are done, which is before the softmax has
+  // read the page data; by the second refill that softmax is over (its weights were needed for the scores in between)
+  constexpr int kMeta = 2 * C::kStages;
+  __shared__ Meta meta[kMeta][2];
+  __shared__ __align__(8) uint64_t bar_k_full[C::kStages], bar_k_empty[C::kStages], bar_v_full[C::kStages], bar_v_empty[C::kStages];
+  __shared__ __align__(8) uint64_t bar_q[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int found;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = (int)(c.heads / c.kv_heads), H = (int)c.kv_heads;
+  long long budget = 2000000000ll;
+
+  // ---- which rows: sequence s owns the row tiles [floor(q_start[s] group / 256) + s, the same of s + 1) of the grid ----
+  const int slots = gridDim.x / H;
+  const int head = blockIdx.x % H, slot = slots - 1 - (int)(blockIdx.x / H);     // the long causal tiles first
+  auto first_slot = [&](int s) { return (int)((int64_t)__ldg(c.q_start + s) * group / kCtaRows) + s; };
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  {
+    int n = 0;
+    for (int s = threadIdx.x; s < c.seqs; s += kThreads) n += first_slot(s) <= slot;
+    if (n) atomicAdd(&found, n);
+  }
+  __syncthreads();
+  const int seq = found - 1;
+  if (seq < 0) return;
+  const int q0 = __ldg(c.q_start + seq), q1 = __ldg(c.q_start + seq + 1), kv_raw = __ldg(c.kv_len + seq);
+  const int tile = slot - first_slot(seq);
+  if (q0 < 0 || q1 > c.tokens || q1 < q0) {
+    if (threadIdx.x == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+    return;
+  }
+  const int n = q1 - q0, rows_all = n * group, row0 = tile * kCtaRows;
+  if (tile < 0 || row0 >= rows_all) return;                     // tile < 0: q_start runs backwards
+  const int kv = (int)min((int64_t)max(kv_raw, 0), c.table_width * kPageTokens);
+  auto limit_of = [&](int r) { return c.causal ? min(kv, kv_raw - n + r / group + 1) : kv; };
+  const int hi = max(0, limit_of(min(rows_all, row0 + kCtaRows) - 1));
+  const int steps_all = (hi + kTileTokens - 1) / kTileTokens;
+  const int per = (steps_all + splits - 1) / splits, j0 = (int)blockIdx.y * per;
+  const int steps = max(0, min(per, steps_all - j0));
+  const bool two = rows_all - row0 > kTileRows;                 // the second tile has rows
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(smem_u32(&bar_k_full[i]), kProducers);
+      mbar_init(smem_u32(&bar_v_full[i]), kProducers);
+      mbar_init(smem_u32(&bar_k_empty[i]), 1);
+      mbar_init(smem_u32(&bar_v_empty[i]), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&bar_q[g]), 4);
+      mbar_init(smem_u32(&bar_s[g]), 2);                        // the MMAs' commit, and the issuing thread itself (page data)
+      mbar_init(smem_u32(&bar_p[g]), 4);
+      mbar_init(smem_u32(&bar_o[g]), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tcgen05_alloc(smem_u32(&tmem_slot), 512);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t q_at = base, k_at = base + 2 * C::kQBytes, v_at = k_at + C::kStages * C::kKBytes;
+
+  if (warp < 8) {
+    // ---------------- softmax: thread = row ----------------
+    const int g = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
+    const int r = row0 + g * kTileRows + in_tile;
+    const bool live = r < rows_all;
+    if (g == 1 && !two) {
+    } else {
+      const int64_t tok = q0 + r / group;
+      const int hd = head * group + r % group;
+      float unit = 1.f;
+      {
+        const T* row = static_cast<const T*>(c.q) + tok * c.q_ts + (int64_t)hd * c.q_hs;
+        uint4 raw[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) raw[i] = live ? *reinterpret_cast<const uint4*>(row + 8 * i) : make_uint4(0, 0, 0, 0);
+        float inv = 1.f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          float m = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { const float2 f = unpack2(w[e], T{}); m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y))); }
+          }
+          const int e = min(max((int)(__float_as_uint(m) >> 23), 2), 252);       // see cache_attend.cu
+          unit = __uint_as_float((uint32_t)e << 23);
+          inv = __uint_as_float((uint32_t)(254 - e) << 23);
+        }
+        const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;                   // the maximum is taken before the scale
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+              const float2 f = unpack2(w[e], T{});
+              w[e] = pack2(f.x * inv, f.y * inv, __half{});
+            }
+            w[e] ^= flip;
+          }
+          uint8_t* dst = gen + (q_at - base) + g * C::kQBytes + (i / 8) * (kTileRows * 128) + in_tile * 128 + (((i & 7) ^ (in_tile & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_q[g]));
+      }
+      const float coef = unit * fabsf(c.scale) * 1.4426950408889634f;
+      const int limit = live ? limit_of(r) : 0x7fffffff;
+      int least = limit;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(~0u, least, o));
+      const uint32_t s_col = tmem + ((uint32_t)(quad * 32) << 16) + C::kTmemS + 128 * g;
+      const uint32_t o_col = tmem + ((uint32_t)(quad * 32) << 16) + C::kTmemO + D * g;
+      float M = -INFINITY, L = 0.f;
+
+      for (int j = 0; j < steps; ++j) {
+        const int tok0 = (j0 + j) * kTileTokens;
+        mbar_wait(smem_u32(&bar_s[g]), j & 1, budget, &g_attend_many_status, 4);
+        __syncwarp();
+        tcgen05_fence_after();
+        const bool masked = tok0 + kTileTokens > least;
+        float top = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const Meta md = meta[j % kMeta][p];
+          float m = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            tcgen05_ld_32x32b_x32(s_col + p * 64 + h * 32, v);
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (tok0 + p * 64 + h * 32 + i < limit) m = fmaxf(m, __uint_as_float(v[i]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) m = fmaxf(m, __uint_as_float(v[i]));
+            }
+          }
+          // a page of masked scores alone leaves m at -inf: -inf * 0 would be NaN
+          top = fmaxf(top, m == -INFINITY ? m : fmaf(m, coef * md.ks, md.log2_vs));
+        }
+        const bool raise = top > M + kRaise || (M == -INFINITY && top > M);
+        if (__any_sync(~0u, raise)) {
+          const float to = fmaxf(M, top);
+          const float f = to == -INFINITY ? 1.f : exp2f(M - to);
+          M = to;
+          L *= f;
+          if (j > 0) {
+            mbar_wait(smem_u32(&bar_o[g]), (j - 1) & 1, budget, &g_attend_many_status, 5);
+            __syncwarp();
+            tcgen05_fence_after();
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+              uint32_t v[32];
+              tcgen05_ld_32x32b_x32(o_col + d, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tcgen05_st_32x32b_x32_nowait(o_col + d, v);
+            }
+            tcgen05_wait_st();
+          }
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const Meta md = meta[j % kMeta][p];
+          const float k = coef * md.ks, off = md.log2_vs - ref;
+          float sum = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32], w[16];
+            tcgen05_ld_32x32b_x32(s_col + p * 64 + h * 32, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float x = fmaf(__uint_as_float(v[i]), k, off);
+              if (masked && tok0 + p * 64 + h * 32 + i >= limit) x = -INFINITY;
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(x));
+              sum += x;
+              v[i] = __float_as_uint(x);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), __half{});
+            tmem_st16(s_col + (p * 2 + h) * 16, w);             // over scores that have been read
+          }
+          L += sum * md.inv_vs;
+        }
+        tcgen05_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p[g]));
+      }
+
+      // ---- result ----
+      if (steps > 0) {
+        mbar_wait(smem_u32(&bar_o[g]), (steps - 1) & 1, budget, &g_attend_many_status, 6);
+        __syncwarp();
+        tcgen05_fence_after();
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      float* part = partial + ((int64_t)blockIdx.y * c.tokens * c.heads + tok * c.heads + hd) * (D + 4);
+      T* out = static_cast<T*>(c.out) + tok * c.o_ts + (int64_t)hd * c.o_hs;
+      if (splits > 1 && live) { part[D] = M; part[D + 1] = L; }
+#pragma unroll
+      for (int d = 0; d < D; d += 32) {
+        uint32_t v[32];
+        if (steps > 0) {
+          tcgen05_ld_32x32b_x32(o_col + d, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
+        }
+        if (!live) continue;
+        if (splits > 1) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(part + d + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = L == 0.f ? 0.f : __uint_as_float(v[8 * i + e]) * inv;
+            store8(out + d + 8 * i, f);
+          }
+        }
+      }
+      tcgen05_fence_before();
+    }
+  } else if (warp == 8) {
+    // ---------------- MMA issue ----------------
+    if (lane == 0) {
+      const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTileTokens >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+      const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+      const int tiles = two ? 2 : 1;
+      auto scores = [&](int g, int j) {
+        const int st = j % C::kStages;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ss(tmem + C::kTmemS + 128 * g, make_desc(q_at + g * C::kQBytes + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128),
+                     make_desc(k_at + st * C::kKBytes + (k / 4) * (kTileTokens * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128), idesc_s, k > 0);
+        tcgen05_commit(smem_u32(&bar_s[g]));
+        mbar_arrive(smem_u32(&bar_s[g]));
+        if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_k_empty[st]));
+      };
+      for (int g = 0; g < tiles; ++g) mbar_wait(smem_u32(&bar_q[g]), 0, budget, &g_attend_many_status, 1);
+      if (steps > 0) {
+        mbar_wait(smem_u32(&bar_k_full[0]), 0, budget, &g_attend_many_status, 2);
+        tcgen05_fence_after();
+        for (int g = 0; g < tiles; ++g) scores(g, 0);
+      }
+      for (int j = 0; j < steps; ++j) {
+        const int st = j % C::kStages, par = (j / C::kStages) & 1;
+        mbar_wait(smem_u32(&bar_v_full[st]), par, budget, &g_attend_many_status, 2);
+        for (int g = 0; g < tiles; ++g) {
+          mbar_wait(smem_u32(&bar_p[g]), j & 1, budget, &g_attend_many_status, 3);
+          tcgen05_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileTokens / 16; ++k)
+            mma_f16_ts(tmem + C::kTmemO + D * g, tmem + C::kTmemS + 128 * g + 8 * k,
+                       make_desc(v_at + st * C::kVBytes + (k / 4) * (D * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128), idesc_o, j > 0 || k > 0);
+          tcgen05_commit(smem_u32(&bar_o[g]));
+          if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_v_empty[st]));
+          if (j + 1 < steps) {
+            if (g == 0) {
+              mbar_wait(smem_u32(&bar_k_full[(j + 1) % C::kStages]), ((j + 1) / C::kStages) & 1, budget, &g_attend_many_status, 2);
+              tcgen05_fence_after();
+            }
+            scores(g, j + 1);                                   // MMAs run in order: the weights in these columns are read by then
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- producers ----------------
+    const int pt = threadIdx.x - 9 * 32;                        // 0 .. 127
+    constexpr int kChunks = D / 16;                             // 16-byte pieces of a key row
+    constexpr int kKPer = kTileTokens * kChunks / (kProducers * 32), kVPer = 2 * D * 4 / (kProducers * 32);
+    const int* table = c.table + (int64_t)seq * c.table_stride;
+    const uint8_t* kpool = static_cast<const uint8_t*>(c.k_pages);
+    const uint8_t* vpool = static_cast<const uint8_t*>(c.v_pages);
+    constexpr int64_t kPageHead = kPageTokens * D;
+    // page p of step j as an offset of (page, head) or -1
+    auto look_up = [&](int j, int64_t (&ph)[2]) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int pg = (j0 + j) * 2 + p;
+        ph[p] = -1;
+        if (j < steps && (int64_t)pg * kPageTokens < kv) {
+          const int id = __ldg(table + pg);
+          if (id >= 0 && id < c.pages) ph[p] = (int64_t)id * H + head;
+          else if (pt == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+        }
+      }
+    };
+    // lanes: 8 rows x 4 pieces, a quarter warp = 8 rows of one piece: the swizzle spreads its stores over all banks
+    auto place = [&](int i, int pieces, int& row, int& piece) {
+      const int u = i * kProducers + (pt >> 5);                 // group of 8 rows x 4 pieces
+      row = (u / (pieces / 4)) * 8 + (lane & 7);
+      piece = (u % (pieces / 4)) * 4 + (lane >> 3);
+    };
+    uint4 kr[kKPer], vr[kVPer];
+    Meta mine{};
+    auto load_k = [&](const int64_t (&ph)[2]) {
+#pragma unroll
+      for (int i = 0; i < kKPer; ++i) {
+        int row, piece;
+        place(i, kChunks, row, piece);
+        const int64_t at = ph[i / (kKPer / 2)];                 // = row / 64
+        kr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(kpool + at * kPageHead + (row & 63) * D + piece * 16) : make_uint4(0, 0, 0, 0);
+      }
+      if (pt < 2) {
+        const int64_t at = ph[pt];
+        if (at >= 0) {
+          const float vs = fmaxf(__ldg(c.v_scale + at), 5.421010862e-20f);       // see cache_attend.cu
+          mine = {__ldg(c.k_scale + at), log2f(vs), 1.f / vs, 0.f};
+        } else {
+          mine = {0.f, -INFINITY, 0.f, 0.f};                    // nothing there: no weight
+        }
+      }
+    };
+    auto load_v = [&](const int64_t (&ph)[2]) {
+#pragma unroll
+      for (int i = 0; i < kVPer; ++i) {
+        int row, piece;                                         // row: page * D + dim
+        place(i, 4, row, piece);
+        const int64_t at = ph[i / (kVPer / 2)];                 // = row / D
+        vr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(vpool + at * kPageHead + (row % D) * kPageTokens + piece * 16) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto widen = [&](uint32_t w, uint32_t& lo, uint32_t& hi) { lo = e4m3_lo(w); hi = e4m3_hi(w); };
+    // 16 codes -> 32 bytes at 16-byte pieces 2 piece, 2 piece + 1 of a row of 128-byte blocks
+    auto put = [&](uint8_t* block0, int block_bytes, int row, int piece, const uint4& x) {
+      uint4 a, b;
+      widen(x.x, a.x, a.y), widen(x.y, a.z, a.w), widen(x.z, b.x, b.y), widen(x.w, b.z, b.w);
+      uint8_t* p = block0 + (piece >> 2) * block_bytes + row * 128;
+      const int o = (piece & 3) * 2;
+      *reinterpret_cast<uint4*>(p + ((o ^ (row & 7)) << 4)) = a;
+      *reinterpret_cast<uint4*>(p + (((o + 1) ^ (row & 7)) << 4)) = b;
+    };
+    int64_t now[2], next[2];
+    look_up(0, now);
+    if (steps > 0) { load_k(now); load_v(now); }
+    look_up(1, next);
+    for (int j = 0; j < steps; ++j) {
+      const int st = j % C::kStages, par = ((j / C::kStages) & 1) ^ 1;
+      mbar_wait(smem_u32(&bar_k_empty[st]), par, budget, &g_attend_many_status, 7);
+      __syncwarp();
+      {
+        uint8_t* dst = gen + (k_at - base) + st * C::kKBytes;
+#pragma unroll
+        for (int i = 0; i < kKPer; ++i) {
+          int row, piece;
+          place(i, kChunks, row, piece);
+          put(dst, kTileTokens * 128, row, piece, kr[i]);
+        }
+        if (pt < 2) meta[j % kMeta][pt] = mine;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_k_full[st]));
+      if (j + 1 < steps) load_k(next);
+      mbar_wait(smem_u32(&bar_v_empty[st]), par, budget, &g_attend_many_status, 8);
+      __syncwarp();
+      {
+        uint8_t* dst = gen + (v_at - base) + st * C::kVBytes;
+        const int tok0 = (j0 + j) * kTileTokens;
+        const bool tail = tok0 + kTileTokens > kv;              // bytes behind the end may be anything: zeros instead
+#pragma unroll
+        for (int i = 0; i < kVPer; ++i) {
+          int row, piece;
+          place(i, 4, row, piece);
+          const int page = i / (kVPer / 2), dim = row % D;
+          uint4 x = vr[i];
+          if (tail) {
+            const int live = kv - (tok0 + page * 64 + piece * 16);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int l = live - 4 * e;
+              w[e] &= l >= 4 ? ~0u : l <= 0 ? 0u : ~0u >> (8 * (4 - l));
+            }
+          }
+          put(dst + page * (D * 128), 0, dim, piece, x);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_v_full[st]));
+      if (j + 1 < steps) load_v(next);
+      look_up(j + 2, next);
+    }
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tcgen05_fence_after();
+    tcgen05_dealloc(tmem, 512);
+  }
+}
+
+// Joins the splits of a row: one warp per (token, head).
+template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_join_kernel(const ob::CacheAttendCall c, const float* partial, int splits) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = c.tokens * c.heads;
+  if (row >= rows) return;
+  const int t = (int)(row / c.heads);
+  int first = 0;
+  for (int s0 = 0; s0 <= c.seqs; s0 += 32) first += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && __ldg(c.q_start + min((int64_t)s0 + lane, c.seqs)) <= t));
+  if (first < 1 || first > c.seqs) return;                      // padding: not written
+  const int q0 = __ldg(c.q_start + first - 1), q1 = __ldg(c.q_start + first);
+  if (q0 < 0 || q1 > c.tokens) return;
+  const float* p = partial + row * (D + 4);
+  const int64_t step = rows * (D + 4);
+  float M = -INFINITY;
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, p[s * step + D]);
+  const float R = M == -INFINITY ? 0.f : M;
+  float L = 0.f, o[D / 32] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float f = exp2f(p[s * step + D] - R);
+    L += f * p[s * step + D + 1];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) o[e] += f * p[s * step + lane + 32 * e];
+  }
+  T* out = static_cast<T*>(c.out) + t * c.o_ts + (row % c.heads) * c.o_hs;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) out[lane + 32 * e] = from_f32<T>(L == 0.f ? 0.f : o[e] / L);
+}
+
+int64_t many_slots(const ob::CacheAttendCall& c) { return c.tokens * (c.heads / c.kv_heads) / kCtaRows + c.seqs; }
+
+int many_splits(const ob::CacheAttendCall& c) {
+  const int64_t ctas = many_slots(c) * c.kv_heads, sms = ob::sm_count();
+  if (ctas >= 2 * sms) return 1;
+  const int64_t most = std::max<int64_t>(1, (c.table_width + 15) / 16);          // at least 8 steps of 128 tokens each
+  return (int)std::min<int64_t>({(2 * sms + ctas - 1) / ctas, most, 64});
+}
+
+template <typename T, int D> cudaError_t launch_many(const ob::CacheAttendCall& c, void* workspace, cudaStream_t stream) {
+  const int splits = many_splits(c);
+  float* partial = static_cast<float*>(workspace);
+  cudaError_t e = cudaFuncSetAttribute(ob_attend_many_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  ob_attend_many_kernel<T, D><<<dim3((unsigned)(many_slots(c) * c.kv_heads), splits), kThreads, Cfg<D>::kSmem, stream>>>(c, partial, splits);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || splits == 1) return e;
+  ob_attend_join_kernel<T, D><<<(unsigned)((c.tokens * c.heads + 7) / 8), 256, 0, stream>>>(c, partial, splits);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+namespace ob {
+
+int64_t cache_attend_many_workspace(const CacheAttendCall& c) {
+  const int splits = many_splits(c);
+  return splits == 1 ? 0 : splits * c.tokens * c.heads * (c.head_dim + 4) * 4;
+}
+
+cudaError_t launch_cache_attend_many(const CacheAttendCall& c, void* workspace, cudaStream_t stream) {
+  if (c.bf16) return c.head_dim == 64 ? launch_many<__nv_bfloat16, 64>(c, workspace, stream) : launch_many<__nv_bfloat16, 128>(c, workspace, stream);
+  return c.head_dim == 64 ? launch_many<__half, 64>(c, workspace, stream) : launch_many<__half, 128>(c, workspace, stream);
+}
+
+cudaError_t read_attend_many_status(int* out) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_attend_many_status, sizeof(int));
+  if (e != cudaSuccess || *out == 0) return e;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_attend_many_status, &zero, sizeof(int));
+}
+
+}  // namespace ob

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kRotThreads) ob_cache_append_kernel(const Appe
   const int before = kv - n;                                  // may be negative: the first -before tokens have no place
   const int block = max(before, 0) / kPageTokens + slot - first_slot(seq);
   const int base = block * kPageTokens;
-  if (base >= kv) return;
+  if (block < 0 || base >= kv) return;                        // block < 0: q_start runs backwards
   const int page = block < b.table_width ? b.table[(int64_t)seq * b.table_stride + block] : -1;
   if (q0 < 0 || q1 > a.tokens || page < 0 || page >= a.pages) {
     if (tid == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);

@@ -2,7 +2,7 @@
 //
 // One CTA owns 256 query rows of a cache head -- the rows of all heads of its group, token by token, so that a group shares
 // the keys -- as two tiles of 128, and walks over the cached tokens 128 at a time:
-//   * producers (4 warps) fetch two pages' keys and values with 16-byte loads one step ahead, widen e4m3 to fp16 (exact) and
+//   * producers (3 warps) fetch two pages' keys and values with 16-byte loads one step ahead, widen e4m3 to fp16 (exact) and
 //     store them as K-major operands with the 128-byte swizzle. The pages' layout makes both K-major: keys (token, dim) for
 //     S = Q K^T, values (dim, token) for O += P V. Widening once per CTA costs what a TMA load of fp16 would cost in shared
 //     memory, and the cache is read at 8 bits;
@@ -30,7 +30,7 @@ using namespace ob_ptx;
 __device__ int g_attend_many_status;
 
 constexpr int kTileRows = 128, kCtaRows = 256, kTileTokens = 128;
-constexpr int kProducers = 4;                                   // warps
+constexpr int kProducers = 3;                                   // warps
 constexpr int kThreads = 32 * (8 + 1 + kProducers);
 constexpr float kRaise = 8.f;                                   // log2 of the largest weight before the reference is raised
 
@@ -51,11 +51,64 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// 32 columns of this warp's lanes, without the wait
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+// the wait, with the loaded registers as operands: nothing that uses them can be moved before it
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[128]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[i]));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
                  "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
+// two fp32 at a time
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1)
 ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   using C = Cfg<D>;
@@ -189,27 +242,32 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
         mbar_wait(smem_u32(&bar_s[g]), j & 1, budget, &g_attend_many_status, 4);
         __syncwarp();
         tcgen05_fence_after();
-        const bool masked = tok0 + kTileTokens > least;
+        uint32_t v[kTileTokens];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) tmem_ld32(s_col + h * 32, v + h * 32);
+        const Meta md[2] = {meta[j % kMeta][0], meta[j % kMeta][1]};
+        // never 0: a masked score is -inf, and -inf * 0 would be NaN
+        const float k[2] = {fmaxf(coef * md[0].ks, 1e-37f), fmaxf(coef * md[1].ks, 1e-37f)};
+        tmem_landed(v);
+        if (tok0 + kTileTokens > least) {
+#pragma unroll
+          for (int i = 0; i < kTileTokens; ++i)
+            if (tok0 + i >= limit) v[i] = 0xFF800000u;
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const Meta md = meta[j % kMeta][p];
-          float m = -INFINITY;
+          float m[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            tcgen05_ld_32x32b_x32(s_col + p * 64 + h * 32, v);
-            if (masked) {
+          for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(v[p * 64 + i]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (tok0 + p * 64 + h * 32 + i < limit) m = fmaxf(m, __uint_as_float(v[i]));
-            } else {
+          for (int i = 4; i < 64; i += 8) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) m = fmaxf(m, __uint_as_float(v[i]));
-            }
+            for (int e = 0; e < 4; ++e)
+              m[e] = i + 4 + e < 64 ? fmaxf(m[e], fmaxf(__uint_as_float(v[p * 64 + i + e]), __uint_as_float(v[p * 64 + i + 4 + e])))
+                                    : fmaxf(m[e], __uint_as_float(v[p * 64 + i + e]));
           }
-          // a page of masked scores alone leaves m at -inf: -inf * 0 would be NaN
-          top = fmaxf(top, m == -INFINITY ? m : fmaf(m, coef * md.ks, md.log2_vs));
+          top = fmaxf(top, fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), k[p], md[p].log2_vs));
         }
         const bool raise = top > M + kRaise || (M == -INFINITY && top > M);
         if (__any_sync(~0u, raise)) {
@@ -221,13 +279,13 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
             mbar_wait(smem_u32(&bar_o[g]), (j - 1) & 1, budget, &g_attend_many_status, 5);
             __syncwarp();
             tcgen05_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < D; d += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_col + d, o);
 #pragma unroll
-            for (int d = 0; d < D; d += 32) {
-              uint32_t v[32];
-              tcgen05_ld_32x32b_x32(o_col + d, v);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tcgen05_st_32x32b_x32_nowait(o_col + d, v);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(o_col + d, o);
             }
             tcgen05_wait_st();
           }
@@ -235,26 +293,18 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
         const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const Meta md = meta[j % kMeta][p];
-          const float k = coef * md.ks, off = md.log2_vs - ref;
-          float sum = 0.f;
+          const uint64_t k2 = pair(k[p], k[p]), off2 = pair(md[p].log2_vs - ref, md[p].log2_vs - ref);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32], w[16];
-            tcgen05_ld_32x32b_x32(s_col + p * 64 + h * 32, v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float x = fmaf(__uint_as_float(v[i]), k, off);
-              if (masked && tok0 + p * 64 + h * 32 + i >= limit) x = -INFINITY;
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(x));
-              sum += x;
-              v[i] = __float_as_uint(x);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), __half{});
-            tmem_st16(s_col + (p * 2 + h) * 16, w);             // over scores that have been read
+          for (int i = 0; i < 32; ++i) {
+            const float2 x = unpair(fma2(pair(__uint_as_float(v[p * 64 + 2 * i]), __uint_as_float(v[p * 64 + 2 * i + 1])), k2, off2));
+            const float a = ex2(x.x), b = ex2(x.y);
+            sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
+            v[p * 32 + i] = pack2(a, b, __half{});              // over scores that have been used
           }
-          L += sum * md.inv_vs;
+          tcgen05_st_32x32b_x32_nowait(s_col + p * 32, reinterpret_cast<uint32_t(&)[32]>(v[p * 32]));
+          const float2 sum = unpair(add2(sum2[0], sum2[1]));
+          L += (sum.x + sum.y) * md[p].inv_vs;
         }
         tcgen05_wait_st();
         tcgen05_fence_before();
@@ -346,7 +396,11 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     // ---------------- producers ----------------
     const int pt = threadIdx.x - 9 * 32;                        // 0 .. 127
     constexpr int kChunks = D / 16;                             // 16-byte pieces of a key row
-    constexpr int kKPer = kTileTokens * kChunks / (kProducers * 32), kVPer = 2 * D * 4 / (kProducers * 32);
+    // work in units of 8 rows x 4 pieces, one per warp and turn
+    constexpr int kUnits = kTileTokens * kChunks / 32;          // of the keys, and of the values: 2 D rows of 4 pieces
+    constexpr int kTurns = (kUnits + kProducers - 1) / kProducers;
+    static_assert(kUnits == 2 * D * 4 / 32, "keys and values are the same bytes");
+    const int pw = pt >> 5;
     const int* table = c.table + (int64_t)seq * c.table_stride;
     const uint8_t* kpool = static_cast<const uint8_t*>(c.k_pages);
     const uint8_t* vpool = static_cast<const uint8_t*>(c.v_pages);
@@ -365,19 +419,20 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
       }
     };
     // lanes: 8 rows x 4 pieces, a quarter warp = 8 rows of one piece: the swizzle spreads its stores over all banks
-    auto place = [&](int i, int pieces, int& row, int& piece) {
-      const int u = i * kProducers + (pt >> 5);                 // group of 8 rows x 4 pieces
+    auto place = [&](int u, int pieces, int& row, int& piece) {
       row = (u / (pieces / 4)) * 8 + (lane & 7);
       piece = (u % (pieces / 4)) * 4 + (lane >> 3);
     };
-    uint4 kr[kKPer], vr[kVPer];
+    uint4 kr[kTurns], vr[kTurns];
     Meta mine{};
     auto load_k = [&](const int64_t (&ph)[2]) {
 #pragma unroll
-      for (int i = 0; i < kKPer; ++i) {
+      for (int i = 0; i < kTurns; ++i) {
+        const int u = i * kProducers + pw;
+        if (u >= kUnits) break;
         int row, piece;
-        place(i, kChunks, row, piece);
-        const int64_t at = ph[i / (kKPer / 2)];                 // = row / 64
+        place(u, kChunks, row, piece);
+        const int64_t at = u < kUnits / 2 ? ph[0] : ph[1];      // the units of the first page come first
         kr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(kpool + at * kPageHead + (row & 63) * D + piece * 16) : make_uint4(0, 0, 0, 0);
       }
       if (pt < 2) {
@@ -392,10 +447,12 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     };
     auto load_v = [&](const int64_t (&ph)[2]) {
 #pragma unroll
-      for (int i = 0; i < kVPer; ++i) {
+      for (int i = 0; i < kTurns; ++i) {
+        const int u = i * kProducers + pw;
+        if (u >= kUnits) break;
         int row, piece;                                         // row: page * D + dim
-        place(i, 4, row, piece);
-        const int64_t at = ph[i / (kVPer / 2)];                 // = row / D
+        place(u, 4, row, piece);
+        const int64_t at = u < kUnits / 2 ? ph[0] : ph[1];
         vr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(vpool + at * kPageHead + (row % D) * kPageTokens + piece * 16) : make_uint4(0, 0, 0, 0);
       }
     };
@@ -420,9 +477,11 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
       {
         uint8_t* dst = gen + (k_at - base) + st * C::kKBytes;
 #pragma unroll
-        for (int i = 0; i < kKPer; ++i) {
+        for (int i = 0; i < kTurns; ++i) {
+          const int u = i * kProducers + pw;
+          if (u >= kUnits) break;
           int row, piece;
-          place(i, kChunks, row, piece);
+          place(u, kChunks, row, piece);
           put(dst, kTileTokens * 128, row, piece, kr[i]);
         }
         if (pt < 2) meta[j % kMeta][pt] = mine;
@@ -438,10 +497,12 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
         const int tok0 = (j0 + j) * kTileTokens;
         const bool tail = tok0 + kTileTokens > kv;              // bytes behind the end may be anything: zeros instead
 #pragma unroll
-        for (int i = 0; i < kVPer; ++i) {
+        for (int i = 0; i < kTurns; ++i) {
+          const int u = i * kProducers + pw;
+          if (u >= kUnits) break;
           int row, piece;
-          place(i, 4, row, piece);
-          const int page = i / (kVPer / 2), dim = row % D;
+          place(u, 4, row, piece);
+          const int page = u < kUnits / 2 ? 0 : 1, dim = row % D;
           uint4 x = vr[i];
           if (tail) {
             const int live = kv - (tok0 + page * 64 + piece * 16);

@@ -2,7 +2,7 @@
 //
 // One CTA owns 256 query rows of a cache head -- the rows of all heads of its group, token by token, so that a group shares
 // the keys -- as two tiles of 128, and walks over the cached tokens 128 at a time:
-//   * producers (3 warps) fetch two pages' keys and values with 16-byte loads one step ahead, widen e4m3 to fp16 (exact) and
+//   * producers (7 warps) fetch two pages' keys and values with 16-byte loads one step ahead, widen e4m3 to fp16 (exact) and
 //     store them as K-major operands with the 128-byte swizzle. The pages' layout makes both K-major: keys (token, dim) for
 //     S = Q K^T, values (dim, token) for O += P V. Widening once per CTA costs what a TMA load of fp16 would cost in shared
 //     memory, and the cache is read at 8 bits;
@@ -30,15 +30,18 @@ using namespace ob_ptx;
 __device__ int g_attend_many_status;
 
 constexpr int kTileRows = 128, kCtaRows = 256, kTileTokens = 128;
-constexpr int kProducers = 3;                                   // warps
+constexpr int kProducers = 7;                                   // warps
 constexpr int kThreads = 32 * (8 + 1 + kProducers);
+// registers: the softmax warps hold a row's 128 scores; 256 threads of either kind share what 512 x 128 were launched with
+constexpr int kSoftmaxRegs = 168, kServiceRegs = 88;
+static_assert(kThreads == 512 && kSoftmaxRegs + kServiceRegs <= 256, "register split");
 constexpr float kRaise = 8.f;                                   // log2 of the largest weight before the reference is raised
 
 template <int D> struct Cfg {
   static constexpr int kQBytes = kTileRows * D * 2;             // per tile
-  static constexpr int kKBytes = kTileTokens * D * 2, kVBytes = kKBytes;
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  static constexpr int kSmem = 2 * kQBytes + kStages * (kKBytes + kVBytes) + 1024;
+  static constexpr int kSlotBytes = kTileTokens * D * 2;        // keys or values of a step as fp16
+  static constexpr int kSlots = D == 64 ? 8 : 4;                // keys in even slots, values in odd ones
+  static constexpr int kSmem = 2 * kQBytes + kSlots * kSlotBytes + 1024;
   static_assert(kSmem <= 226 * 1024, "shared memory");
   static constexpr int kTmemS = 0, kTmemO = 256;                // S / P of tile g at 128 g, O of tile g at 256 + D g
 };
@@ -116,11 +119,11 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   struct Meta { float ks, log2_vs, inv_vs, pad; };
-  // the pages of step j in [j % kMeta]: a stage is filled again when its scores are done, which is before the softmax has
+  // the pages of step j in [j % kMeta]: a slot is filled again when its scores are done, which is before the softmax has
   // read the page data; by the second refill that softmax is over (its weights were needed for the scores in between)
-  constexpr int kMeta = 2 * C::kStages;
+  constexpr int kMeta = C::kSlots;
   __shared__ Meta meta[kMeta][2];
-  __shared__ __align__(8) uint64_t bar_k_full[C::kStages], bar_k_empty[C::kStages], bar_v_full[C::kStages], bar_v_empty[C::kStages];
+  __shared__ __align__(8) uint64_t bar_full[C::kSlots], bar_empty[C::kSlots];
   __shared__ __align__(8) uint64_t bar_q[2], bar_s[2], bar_p[2], bar_o[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int found;
@@ -160,11 +163,9 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   const bool two = rows_all - row0 > kTileRows;                 // the second tile has rows
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(smem_u32(&bar_k_full[i]), kProducers);
-      mbar_init(smem_u32(&bar_v_full[i]), kProducers);
-      mbar_init(smem_u32(&bar_k_empty[i]), 1);
-      mbar_init(smem_u32(&bar_v_empty[i]), 1);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), kProducers);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&bar_q[g]), 4);
@@ -179,10 +180,11 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
-  const uint32_t q_at = base, k_at = base + 2 * C::kQBytes, v_at = k_at + C::kStages * C::kKBytes;
+  const uint32_t q_at = base, ring_at = base + 2 * C::kQBytes;
 
   if (warp < 8) {
     // ---------------- softmax: thread = row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int g = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
     const int r = row0 + g * kTileRows + in_tile;
     const bool live = r < rows_all;
@@ -347,180 +349,162 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
       }
       tcgen05_fence_before();
     }
-  } else if (warp == 8) {
-    // ---------------- MMA issue ----------------
-    if (lane == 0) {
-      const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTileTokens >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-      const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-      const int tiles = two ? 2 : 1;
-      auto scores = [&](int g, int j) {
-        const int st = j % C::kStages;
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+    if (warp == 8) {
+    // ---------------- MMA issue: the warp stays together, one lane's instructions count ----------------
+    const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTileTokens >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+    const int tiles = two ? 2 : 1;
+    const bool first = lane == 0;
+    const uint64_t q_desc = make_desc(q_at, 16, 1024, kLayoutSw128), ring_desc = make_desc(ring_at, 16, 1024, kLayoutSw128);
+    auto wait_full = [&](int item) {
+      mbar_wait(smem_u32(&bar_full[item % C::kSlots]), (item / C::kSlots) & 1, budget, &g_attend_many_status, 2);
+      tcgen05_fence_after();
+    };
+    auto scores = [&](int g, int j) {
+      const int slot = 2 * j % C::kSlots;
+      if (first) {
+        const uint64_t qd = q_desc + (uint64_t)(g * (C::kQBytes >> 4)), kd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + C::kTmemS + 128 * g, make_desc(q_at + g * C::kQBytes + (k / 4) * (kTileRows * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128),
-                     make_desc(k_at + st * C::kKBytes + (k / 4) * (kTileTokens * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128), idesc_s, k > 0);
+          mma_f16_ss(tmem + C::kTmemS + 128 * g, qd + (uint64_t)(((k / 4) * (kTileRows * 128) + (k % 4) * 32) >> 4),
+                     kd + (uint64_t)(((k / 4) * (kTileTokens * 128) + (k % 4) * 32) >> 4), idesc_s, k > 0);
         tcgen05_commit(smem_u32(&bar_s[g]));
         mbar_arrive(smem_u32(&bar_s[g]));
-        if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_k_empty[st]));
-      };
-      for (int g = 0; g < tiles; ++g) mbar_wait(smem_u32(&bar_q[g]), 0, budget, &g_attend_many_status, 1);
-      if (steps > 0) {
-        mbar_wait(smem_u32(&bar_k_full[0]), 0, budget, &g_attend_many_status, 2);
-        tcgen05_fence_after();
-        for (int g = 0; g < tiles; ++g) scores(g, 0);
+        if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
       }
-      for (int j = 0; j < steps; ++j) {
-        const int st = j % C::kStages, par = (j / C::kStages) & 1;
-        mbar_wait(smem_u32(&bar_v_full[st]), par, budget, &g_attend_many_status, 2);
-        for (int g = 0; g < tiles; ++g) {
-          mbar_wait(smem_u32(&bar_p[g]), j & 1, budget, &g_attend_many_status, 3);
-          tcgen05_fence_after();
+      __syncwarp();
+    };
+    for (int g = 0; g < tiles; ++g) mbar_wait(smem_u32(&bar_q[g]), 0, budget, &g_attend_many_status, 1);
+    if (steps > 0) {
+      wait_full(0);
+      for (int g = 0; g < tiles; ++g) scores(g, 0);
+    }
+    for (int j = 0; j < steps; ++j) {
+      const int slot = (2 * j + 1) % C::kSlots;
+      wait_full(2 * j + 1);
+      for (int g = 0; g < tiles; ++g) {
+        mbar_wait(smem_u32(&bar_p[g]), j & 1, budget, &g_attend_many_status, 3);
+        tcgen05_fence_after();
+        if (first) {
+          const uint64_t vd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
 #pragma unroll
           for (int k = 0; k < kTileTokens / 16; ++k)
-            mma_f16_ts(tmem + C::kTmemO + D * g, tmem + C::kTmemS + 128 * g + 8 * k,
-                       make_desc(v_at + st * C::kVBytes + (k / 4) * (D * 128) + (k % 4) * 32, 16, 1024, kLayoutSw128), idesc_o, j > 0 || k > 0);
+            mma_f16_ts(tmem + C::kTmemO + D * g, tmem + C::kTmemS + 128 * g + 8 * k, vd + (uint64_t)(((k / 4) * (D * 128) + (k % 4) * 32) >> 4), idesc_o,
+                       j > 0 || k > 0);
           tcgen05_commit(smem_u32(&bar_o[g]));
-          if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_v_empty[st]));
-          if (j + 1 < steps) {
-            if (g == 0) {
-              mbar_wait(smem_u32(&bar_k_full[(j + 1) % C::kStages]), ((j + 1) / C::kStages) & 1, budget, &g_attend_many_status, 2);
-              tcgen05_fence_after();
-            }
-            scores(g, j + 1);                                   // MMAs run in order: the weights in these columns are read by then
-          }
+          if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
+        }
+        __syncwarp();
+        if (j + 1 < steps) {
+          if (g == 0) wait_full(2 * j + 2);
+          scores(g, j + 1);                                     // MMAs run in order: the weights in these columns are read by then
         }
       }
     }
-    __syncwarp();
-  } else {
-    // ---------------- producers ----------------
-    const int pt = threadIdx.x - 9 * 32;                        // 0 .. 127
-    constexpr int kChunks = D / 16;                             // 16-byte pieces of a key row
-    // work in units of 8 rows x 4 pieces, one per warp and turn
-    constexpr int kUnits = kTileTokens * kChunks / 32;          // of the keys, and of the values: 2 D rows of 4 pieces
+    } else {
+    // ---------------- producers: items 2 j (keys of step j) and 2 j + 1 (values), both by the same code ----------------
+    const int pw = warp - 9;
+    // Work in units of 8 rows x 64 bytes, one per warp and turn: a lane takes 16 bytes, a quarter warp 8 rows, whose
+    // widened halves the swizzle spreads over all banks. An item is two pages; a page's rows are D values of a key or 64 tokens of
+    // a value, 128 bytes of fp16 in a row of a column block.
+    constexpr int kUnits = kTileTokens * D / 512;               // of an item
     constexpr int kTurns = (kUnits + kProducers - 1) / kProducers;
-    static_assert(kUnits == 2 * D * 4 / 32, "keys and values are the same bytes");
-    const int pw = pt >> 5;
+    constexpr int kPageHead = kPageTokens * D;
+    const int row = lane & 7, piece = lane >> 3;
+    const int put0 = row * 128 + (((2 * piece) ^ row) << 4), put1 = row * 128 + (((2 * piece + 1) ^ row) << 4);
     const int* table = c.table + (int64_t)seq * c.table_stride;
-    const uint8_t* kpool = static_cast<const uint8_t*>(c.k_pages);
-    const uint8_t* vpool = static_cast<const uint8_t*>(c.v_pages);
-    constexpr int64_t kPageHead = kPageTokens * D;
-    // page p of step j as an offset of (page, head) or -1
-    auto look_up = [&](int j, int64_t (&ph)[2]) {
+    // Page numbers are fetched two steps ahead, pages an item ahead; nothing is looked at where it is fetched, so that no
+    // fetch is waited for. ids < 0: no page.
+    auto look_up = [&](int j, int (&ids)[2]) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const int pg = (j0 + j) * 2 + p;
-        ph[p] = -1;
-        if (j < steps && (int64_t)pg * kPageTokens < kv) {
-          const int id = __ldg(table + pg);
-          if (id >= 0 && id < c.pages) ph[p] = (int64_t)id * H + head;
-          else if (pt == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
-        }
+        const int64_t pg = (int64_t)(j0 + j) * 2 + p;
+        ids[p] = j < steps && pg * kPageTokens < kv ? __ldg(table + pg) : -2;       // -2: behind the end, not an error
       }
     };
-    // lanes: 8 rows x 4 pieces, a quarter warp = 8 rows of one piece: the swizzle spreads its stores over all banks
-    auto place = [&](int u, int pieces, int& row, int& piece) {
-      row = (u / (pieces / 4)) * 8 + (lane & 7);
-      piece = (u % (pieces / 4)) * 4 + (lane >> 3);
-    };
-    uint4 kr[kTurns], vr[kTurns];
-    Meta mine{};
-    auto load_k = [&](const int64_t (&ph)[2]) {
+    auto held = [&](int id) { return id >= 0 && id < c.pages; };
+    auto at_page = [&](int id) { return (int64_t)(held(id) ? id : 0) * H + head; };
+    uint4 x[kTurns];
+    auto load = [&](bool values, const int (&ids)[2]) {
+      const uint8_t* pool = static_cast<const uint8_t*>(values ? c.v_pages : c.k_pages);
+      const bool narrow = values || D == 64;                    // rows of 64 bytes: a unit is 512 in a row
+      const int mine = row * (narrow ? 64 : 128) + piece * 16;
+      const uint8_t* page[2] = {pool + at_page(ids[0]) * kPageHead + mine, pool + at_page(ids[1]) * kPageHead + mine};
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        const int u = i * kProducers + pw;
+        const int u = i * kProducers + pw, v = u % (kUnits / 2);
         if (u >= kUnits) break;
-        int row, piece;
-        place(u, kChunks, row, piece);
-        const int64_t at = u < kUnits / 2 ? ph[0] : ph[1];      // the units of the first page come first
-        kr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(kpool + at * kPageHead + (row & 63) * D + piece * 16) : make_uint4(0, 0, 0, 0);
-      }
-      if (pt < 2) {
-        const int64_t at = ph[pt];
-        if (at >= 0) {
-          const float vs = fmaxf(__ldg(c.v_scale + at), 5.421010862e-20f);       // see cache_attend.cu
-          mine = {__ldg(c.k_scale + at), log2f(vs), 1.f / vs, 0.f};
-        } else {
-          mine = {0.f, -INFINITY, 0.f, 0.f};                    // nothing there: no weight
-        }
+        x[i] = __ldg(reinterpret_cast<const uint4*>((u < kUnits / 2 ? page[0] : page[1]) + (narrow ? v * 512 : (v >> 1) * 1024 + (v & 1) * 64)));
       }
     };
-    auto load_v = [&](const int64_t (&ph)[2]) {
-#pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const int u = i * kProducers + pw;
-        if (u >= kUnits) break;
-        int row, piece;                                         // row: page * D + dim
-        place(u, 4, row, piece);
-        const int64_t at = u < kUnits / 2 ? ph[0] : ph[1];
-        vr[i] = at >= 0 ? *reinterpret_cast<const uint4*>(vpool + at * kPageHead + (row % D) * kPageTokens + piece * 16) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    auto widen = [&](uint32_t w, uint32_t& lo, uint32_t& hi) { lo = e4m3_lo(w); hi = e4m3_hi(w); };
-    // 16 codes -> 32 bytes at 16-byte pieces 2 piece, 2 piece + 1 of a row of 128-byte blocks
-    auto put = [&](uint8_t* block0, int block_bytes, int row, int piece, const uint4& x) {
-      uint4 a, b;
-      widen(x.x, a.x, a.y), widen(x.y, a.z, a.w), widen(x.z, b.x, b.y), widen(x.w, b.z, b.w);
-      uint8_t* p = block0 + (piece >> 2) * block_bytes + row * 128;
-      const int o = (piece & 3) * 2;
-      *reinterpret_cast<uint4*>(p + ((o ^ (row & 7)) << 4)) = a;
-      *reinterpret_cast<uint4*>(p + (((o + 1) ^ (row & 7)) << 4)) = b;
-    };
-    int64_t now[2], next[2];
+    int now[2], next[2], later[2];                              // pages of the step in hand, of the next and of the one behind
     look_up(0, now);
-    if (steps > 0) { load_k(now); load_v(now); }
     look_up(1, next);
-    for (int j = 0; j < steps; ++j) {
-      const int st = j % C::kStages, par = ((j / C::kStages) & 1) ^ 1;
-      mbar_wait(smem_u32(&bar_k_empty[st]), par, budget, &g_attend_many_status, 7);
-      __syncwarp();
-      {
-        uint8_t* dst = gen + (k_at - base) + st * C::kKBytes;
+    float2 scales{};
+    auto load_scales = [&](const int (&ids)[2]) {               // lanes 0, 1 of the last warp: one page each
+      const int64_t at = at_page(lane == 0 ? ids[0] : ids[1]);
+      scales = make_float2(__ldg(c.k_scale + at), __ldg(c.v_scale + at));
+    };
+    if (steps > 0) { load(false, now); load_scales(now); }
+    for (int item = 0; item < 2 * steps; ++item) {
+      const int slot = item % C::kSlots, j = item >> 1;
+      const bool values = item & 1;
+      if (!held(now[0]) || !held(now[1])) {
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i) {
-          const int u = i * kProducers + pw;
-          if (u >= kUnits) break;
-          int row, piece;
-          place(u, kChunks, row, piece);
-          put(dst, kTileTokens * 128, row, piece, kr[i]);
-        }
-        if (pt < 2) meta[j % kMeta][pt] = mine;
+        for (int i = 0; i < kTurns; ++i)
+          if (!held(i * kProducers + pw < kUnits / 2 ? now[0] : now[1])) x[i] = make_uint4(0, 0, 0, 0);
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_k_full[st]));
-      if (j + 1 < steps) load_k(next);
-      mbar_wait(smem_u32(&bar_v_empty[st]), par, budget, &g_attend_many_status, 8);
-      __syncwarp();
-      {
-        uint8_t* dst = gen + (v_at - base) + st * C::kVBytes;
-        const int tok0 = (j0 + j) * kTileTokens;
-        const bool tail = tok0 + kTileTokens > kv;              // bytes behind the end may be anything: zeros instead
+      const int tok0 = (j0 + j) * kTileTokens;
+      if (values && tok0 + kTileTokens > kv) {                  // bytes behind the end may be anything: zeros instead
 #pragma unroll
         for (int i = 0; i < kTurns; ++i) {
-          const int u = i * kProducers + pw;
-          if (u >= kUnits) break;
-          int row, piece;
-          place(u, 4, row, piece);
-          const int page = u < kUnits / 2 ? 0 : 1, dim = row % D;
-          uint4 x = vr[i];
-          if (tail) {
-            const int live = kv - (tok0 + page * 64 + piece * 16);
-            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+          const int live = kv - (tok0 + (i * kProducers + pw < kUnits / 2 ? 0 : kPageTokens) + piece * 16);
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x[i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int l = live - 4 * e;
-              w[e] &= l >= 4 ? ~0u : l <= 0 ? 0u : ~0u >> (8 * (4 - l));
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int l = live - 4 * e;
+            w[e] &= l >= 4 ? ~0u : l <= 0 ? 0u : ~0u >> (8 * (4 - l));
           }
-          put(dst + page * (D * 128), 0, dim, piece, x);
         }
+      }
+      if (!values && pw == kProducers - 1 && lane < 2) {
+        const int id = lane == 0 ? now[0] : now[1];
+        const float vs = fmaxf(scales.y, 5.421010862e-20f);     // see cache_attend.cu
+        meta[j % kMeta][lane] = held(id) ? Meta{scales.x, __log2f(vs), __frcp_rn(vs), 0.f} : Meta{0.f, -INFINITY, 0.f, 0.f};   // no page: no weight
+        if (!held(id) && id != -2) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+      }
+      mbar_wait(smem_u32(&bar_empty[slot]), ((item / C::kSlots) & 1) ^ 1, budget, &g_attend_many_status, 7);
+      __syncwarp();
+      uint8_t* dst = gen + (ring_at - base) + slot * C::kSlotBytes;
+      const bool narrow = values || D == 64;
+      // keys: rows of both pages below each other, a column block for each 64 dims; values: a column block for each page
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int u = i * kProducers + pw;
+        if (u >= kUnits) break;
+        uint8_t* at = dst + (narrow ? u * 1024 : (u >> 1) * 1024 + (u & 1) * (kTileTokens * 128));
+        uint4 a, b;
+        a.x = e4m3_lo(x[i].x), a.y = e4m3_hi(x[i].x), a.z = e4m3_lo(x[i].y), a.w = e4m3_hi(x[i].y);
+        b.x = e4m3_lo(x[i].z), b.y = e4m3_hi(x[i].z), b.z = e4m3_lo(x[i].w), b.w = e4m3_hi(x[i].w);
+        *reinterpret_cast<uint4*>(at + put0) = a;
+        *reinterpret_cast<uint4*>(at + put1) = b;
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_v_full[st]));
-      if (j + 1 < steps) load_v(next);
-      look_up(j + 2, next);
+      if (lane == 0) mbar_arrive(smem_u32(&bar_full[slot]));
+      if (!values) {
+        load(true, now);
+        look_up(j + 2, later);
+      } else {
+        now[0] = next[0], now[1] = next[1], next[0] = later[0], next[1] = later[1];
+        if (j + 1 < steps) {
+          load(false, now);
+          if (pw == kProducers - 1 && lane < 2) load_scales(now);
+        }
+      }
+    }
     }
   }
   __syncthreads();

@@ -6,8 +6,8 @@
 //     store them as K-major operands with the 128-byte swizzle. The pages' layout makes both K-major: keys (token, dim) for
 //     S = Q K^T, values (dim, token) for O += P V. Widening once per CTA costs what a TMA load of fp16 would cost in shared
 //     memory, and the cache is read at 8 bits;
-//   * one thread issues tcgen05.mma (M = 128, fp32 accumulators in tensor memory): S of one tile is computed while the other
-//     tile's softmax runs;
+//   * one warp issues tcgen05.mma (M = 128, fp32 accumulators in tensor memory): the products of one tile run while the other
+//     tile's softmax does;
 //   * softmax (4 warps per tile, thread = row): the row's scores are read from tensor memory, the weights go back as fp16 over
 //     the scores' own columns and are the A operand of the second product. The running maximum is only raised, and O
 //     multiplied, when it would otherwise let a weight pass 2^8: the sums are fp32, so a lower reference costs nothing.
@@ -46,6 +46,12 @@ template <int D> struct Cfg {
   static constexpr int kTmemS = 0, kTmemO = 256;                // S / P of tile g at 128 g, O of tile g at 256 + D g
 };
 
+// true in exactly one lane of a converged warp (the same lane every time)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -72,6 +78,12 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&r)[128]) {
 #pragma unroll
   for (int i = 0; i < 128; ++i) asm volatile("" : "+r"(r[i]));
 }
+// scores from column `seen` on become -inf
+__device__ __forceinline__ void hide(uint32_t (&v)[128], int seen) {
+#pragma unroll
+  for (int i = 0; i < 128; ++i)
+    if (i >= seen) v[i] = 0xFF800000u;
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -85,27 +97,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
                  "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-// two fp32 at a time
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -118,13 +109,13 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  struct Meta { float ks, log2_vs, inv_vs, pad; };
+  struct Meta { float ks, vs; };                                // of a page; vs < 0: there is none
   // the pages of step j in [j % kMeta]: a slot is filled again when its scores are done, which is before the softmax has
   // read the page data; by the second refill that softmax is over (its weights were needed for the scores in between)
   constexpr int kMeta = C::kSlots;
   __shared__ Meta meta[kMeta][2];
   __shared__ __align__(8) uint64_t bar_full[C::kSlots], bar_empty[C::kSlots];
-  __shared__ __align__(8) uint64_t bar_q[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ __align__(8) uint64_t bar_q[2], bar_s[2], bar_p[2][2], bar_o[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int found;
 
@@ -170,7 +161,8 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&bar_q[g]), 4);
       mbar_init(smem_u32(&bar_s[g]), 2);                        // the MMAs' commit, and the issuing thread itself (page data)
-      mbar_init(smem_u32(&bar_p[g]), 4);
+      mbar_init(smem_u32(&bar_p[g][0]), 4);
+      mbar_init(smem_u32(&bar_p[g][1]), 4);
       mbar_init(smem_u32(&bar_o[g]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -244,18 +236,17 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
         mbar_wait(smem_u32(&bar_s[g]), j & 1, budget, &g_attend_many_status, 4);
         __syncwarp();
         tcgen05_fence_after();
+        const bool masked = tok0 + kTileTokens > least;
         uint32_t v[kTileTokens];
 #pragma unroll
         for (int h = 0; h < 4; ++h) tmem_ld32(s_col + h * 32, v + h * 32);
-        const Meta md[2] = {meta[j % kMeta][0], meta[j % kMeta][1]};
         // never 0: a masked score is -inf, and -inf * 0 would be NaN
+        const Meta md[2] = {meta[j % kMeta][0], meta[j % kMeta][1]};
         const float k[2] = {fmaxf(coef * md[0].ks, 1e-37f), fmaxf(coef * md[1].ks, 1e-37f)};
+        // no page: no weight
+        const float log2_vs[2] = {md[0].vs < 0.f ? -INFINITY : __log2f(md[0].vs), md[1].vs < 0.f ? -INFINITY : __log2f(md[1].vs)};
         tmem_landed(v);
-        if (tok0 + kTileTokens > least) {
-#pragma unroll
-          for (int i = 0; i < kTileTokens; ++i)
-            if (tok0 + i >= limit) v[i] = 0xFF800000u;
-        }
+        if (masked) hide(v, limit - tok0);
         float top = -INFINITY;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -263,13 +254,12 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(v[p * 64 + i]);
 #pragma unroll
-          for (int i = 4; i < 64; i += 8) {
+          for (int i = 4; i < 60; i += 8)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              m[e] = i + 4 + e < 64 ? fmaxf(m[e], fmaxf(__uint_as_float(v[p * 64 + i + e]), __uint_as_float(v[p * 64 + i + 4 + e])))
-                                    : fmaxf(m[e], __uint_as_float(v[p * 64 + i + e]));
-          }
-          top = fmaxf(top, fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), k[p], md[p].log2_vs));
+            for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fmaxf(__uint_as_float(v[p * 64 + i + e]), __uint_as_float(v[p * 64 + i + 4 + e])));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], __uint_as_float(v[p * 64 + 60 + e]));
+          top = fmaxf(top, fmaf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), k[p], log2_vs[p]));
         }
         const bool raise = top > M + kRaise || (M == -INFINITY && top > M);
         if (__any_sync(~0u, raise)) {
@@ -295,23 +285,22 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
         const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const uint64_t k2 = pair(k[p], k[p]), off2 = pair(md[p].log2_vs - ref, md[p].log2_vs - ref);
-          uint64_t sum2[2] = {0, 0};
+          const float off = log2_vs[p] - ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float2 x = unpair(fma2(pair(__uint_as_float(v[p * 64 + 2 * i]), __uint_as_float(v[p * 64 + 2 * i + 1])), k2, off2));
-            const float a = ex2(x.x), b = ex2(x.y);
-            sum2[i & 1] = add2(sum2[i & 1], pair(a, b));
-            v[p * 32 + i] = pack2(a, b, __half{});              // over scores that have been used
+            const float x = ex2(fmaf(__uint_as_float(v[p * 64 + 2 * i]), k[p], off)), y = ex2(fmaf(__uint_as_float(v[p * 64 + 2 * i + 1]), k[p], off));
+            sum[(2 * i) & 3] += x;
+            sum[(2 * i + 1) & 3] += y;
+            v[p * 32 + i] = pack2(x, y, __half{});              // over scores that have been used
           }
           tcgen05_st_32x32b_x32_nowait(s_col + p * 32, reinterpret_cast<uint32_t(&)[32]>(v[p * 32]));
-          const float2 sum = unpair(add2(sum2[0], sum2[1]));
-          L += (sum.x + sum.y) * md[p].inv_vs;
+          L += md[p].vs < 0.f ? 0.f : __fdividef((sum[0] + sum[1]) + (sum[2] + sum[3]), md[p].vs);
+          tcgen05_wait_st();                                    // the page's weights can be multiplied while the other's are computed
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_p[g][p]));
         }
-        tcgen05_wait_st();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_p[g]));
       }
 
       // ---- result ----
@@ -352,11 +341,13 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
     if (warp == 8) {
-    // ---------------- MMA issue: the warp stays together, one lane's instructions count ----------------
+    // ---------------- MMA issue ----------------
+    // The warp stays converged and only the tcgen05 instructions are predicated on one lane, so that descriptors stay in
+    // uniform registers: 64 cycles per M = N = 128 instruction, the tensor core's own pace, against 100 from a branch on the lane.
     const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTileTokens >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
     const uint32_t idesc_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
     const int tiles = two ? 2 : 1;
-    const bool first = lane == 0;
+    const bool first = elect_one();
     const uint64_t q_desc = make_desc(q_at, 16, 1024, kLayoutSw128), ring_desc = make_desc(ring_at, 16, 1024, kLayoutSw128);
     auto wait_full = [&](int item) {
       mbar_wait(smem_u32(&bar_full[item % C::kSlots]), (item / C::kSlots) & 1, budget, &g_attend_many_status, 2);
@@ -364,17 +355,15 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     };
     auto scores = [&](int g, int j) {
       const int slot = 2 * j % C::kSlots;
-      if (first) {
-        const uint64_t qd = q_desc + (uint64_t)(g * (C::kQBytes >> 4)), kd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
+      const uint64_t qd = q_desc + (uint64_t)(g * (C::kQBytes >> 4)), kd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
+      for (int k = 0; k < D / 16; ++k)
+        if (first)
           mma_f16_ss(tmem + C::kTmemS + 128 * g, qd + (uint64_t)(((k / 4) * (kTileRows * 128) + (k % 4) * 32) >> 4),
                      kd + (uint64_t)(((k / 4) * (kTileTokens * 128) + (k % 4) * 32) >> 4), idesc_s, k > 0);
-        tcgen05_commit(smem_u32(&bar_s[g]));
-        mbar_arrive(smem_u32(&bar_s[g]));
-        if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
-      }
-      __syncwarp();
+      if (first) tcgen05_commit(smem_u32(&bar_s[g]));
+      if (first) mbar_arrive(smem_u32(&bar_s[g]));
+      if (first && g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
     };
     for (int g = 0; g < tiles; ++g) mbar_wait(smem_u32(&bar_q[g]), 0, budget, &g_attend_many_status, 1);
     if (steps > 0) {
@@ -384,22 +373,27 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     for (int j = 0; j < steps; ++j) {
       const int slot = (2 * j + 1) % C::kSlots;
       wait_full(2 * j + 1);
+      if (j + 1 < steps) wait_full(2 * j + 2);
       for (int g = 0; g < tiles; ++g) {
-        mbar_wait(smem_u32(&bar_p[g]), j & 1, budget, &g_attend_many_status, 3);
-        tcgen05_fence_after();
-        if (first) {
-          const uint64_t vd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
+        const uint64_t vd = ring_desc + (uint64_t)(slot * (C::kSlotBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < kTileTokens / 16; ++k)
-            mma_f16_ts(tmem + C::kTmemO + D * g, tmem + C::kTmemS + 128 * g + 8 * k, vd + (uint64_t)(((k / 4) * (D * 128) + (k % 4) * 32) >> 4), idesc_o,
-                       j > 0 || k > 0);
-          tcgen05_commit(smem_u32(&bar_o[g]));
-          if (g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
+        for (int p = 0; p < 2; ++p) {
+          mbar_wait(smem_u32(&bar_p[g][p]), j & 1, budget, &g_attend_many_status, 3);
+          tcgen05_fence_after();
+#pragma unroll
+          for (int k = 4 * p; k < 4 * p + 4; ++k)
+            if (first)
+              mma_f16_ts(tmem + C::kTmemO + D * g, tmem + C::kTmemS + 128 * g + 8 * k, vd + (uint64_t)((p * (D * 128) + (k % 4) * 32) >> 4), idesc_o,
+                         j > 0 || k > 0);
         }
-        __syncwarp();
+        if (first) tcgen05_commit(smem_u32(&bar_o[g]));
+        if (first && g == tiles - 1) tcgen05_commit(smem_u32(&bar_empty[slot]));
         if (j + 1 < steps) {
-          if (g == 0) wait_full(2 * j + 2);
-          scores(g, j + 1);                                     // MMAs run in order: the weights in these columns are read by then
+          // the next scores go over the weights' columns, and instructions on different accumulators are not ordered among
+          // themselves: they wait until the product with those weights is complete (2 % of the kernel's time)
+          mbar_wait(smem_u32(&bar_o[g]), j & 1, budget, &g_attend_many_status, 9);
+          tcgen05_fence_after();
+          scores(g, j + 1);
         }
       }
     }
@@ -415,8 +409,8 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     const int row = lane & 7, piece = lane >> 3;
     const int put0 = row * 128 + (((2 * piece) ^ row) << 4), put1 = row * 128 + (((2 * piece + 1) ^ row) << 4);
     const int* table = c.table + (int64_t)seq * c.table_stride;
-    // Page numbers are fetched two steps ahead, pages an item ahead; nothing is looked at where it is fetched, so that no
-    // fetch is waited for. ids < 0: no page.
+    // Page numbers are fetched two steps ahead, pages one; nothing is looked at where it is fetched, so that no fetch is
+    // waited for. ids < 0: no page.
     auto look_up = [&](int j, int (&ids)[2]) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -426,84 +420,83 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     };
     auto held = [&](int id) { return id >= 0 && id < c.pages; };
     auto at_page = [&](int id) { return (int64_t)(held(id) ? id : 0) * H + head; };
-    uint4 x[kTurns];
-    auto load = [&](bool values, const int (&ids)[2]) {
+    auto load = [&](bool values, const int (&ids)[2], uint4 (&x)[kTurns]) {
       const uint8_t* pool = static_cast<const uint8_t*>(values ? c.v_pages : c.k_pages);
-      const bool narrow = values || D == 64;                    // rows of 64 bytes: a unit is 512 in a row
+      const bool narrow = values || D == 64;                    // rows of 64 bytes: a unit is 512 bytes in a row
       const int mine = row * (narrow ? 64 : 128) + piece * 16;
       const uint8_t* page[2] = {pool + at_page(ids[0]) * kPageHead + mine, pool + at_page(ids[1]) * kPageHead + mine};
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        const int u = i * kProducers + pw, v = u % (kUnits / 2);
-        if (u >= kUnits) break;
-        x[i] = __ldg(reinterpret_cast<const uint4*>((u < kUnits / 2 ? page[0] : page[1]) + (narrow ? v * 512 : (v >> 1) * 1024 + (v & 1) * 64)));
+        const int u = i * kProducers + pw, w = u & (kUnits / 2 - 1);
+        if (u < kUnits) x[i] = __ldg(reinterpret_cast<const uint4*>((u < kUnits / 2 ? page[0] : page[1]) + (narrow ? w * 512 : (w >> 1) * 1024 + (w & 1) * 64)));
       }
+    };
+    const bool scaler = pw == kProducers - 1 && lane < 2;       // two lanes that also fetch the scales, of a page each
+    float2 scales{};
+    auto load_scales = [&](const int (&ids)[2]) {
+      const int64_t at = at_page(lane == 0 ? ids[0] : ids[1]);
+      scales = make_float2(__ldg(c.k_scale + at), __ldg(c.v_scale + at));
     };
     int now[2], next[2], later[2];                              // pages of the step in hand, of the next and of the one behind
     look_up(0, now);
     look_up(1, next);
-    float2 scales{};
-    auto load_scales = [&](const int (&ids)[2]) {               // lanes 0, 1 of the last warp: one page each
-      const int64_t at = at_page(lane == 0 ? ids[0] : ids[1]);
-      scales = make_float2(__ldg(c.k_scale + at), __ldg(c.v_scale + at));
-    };
-    if (steps > 0) { load(false, now); load_scales(now); }
-    for (int item = 0; item < 2 * steps; ++item) {
-      const int slot = item % C::kSlots, j = item >> 1;
-      const bool values = item & 1;
-      if (!held(now[0]) || !held(now[1])) {
+    look_up(2, later);
+    uint4 x[2][kTurns];
+    if (steps > 0) {
+      load(false, now, x[0]);
+      load(true, now, x[1]);
+      if (scaler) load_scales(now);
+    }
+    for (int j = 0; j < steps; ++j) {
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i)
-          if (!held(i * kProducers + pw < kUnits / 2 ? now[0] : now[1])) x[i] = make_uint4(0, 0, 0, 0);
-      }
-      const int tok0 = (j0 + j) * kTileTokens;
-      if (values && tok0 + kTileTokens > kv) {                  // bytes behind the end may be anything: zeros instead
+      for (int values = 0; values < 2; ++values) {
+        const int item = 2 * j + values, slot = item % C::kSlots;
+        if (!held(now[0]) || !held(now[1])) {
+          if ((!held(now[0]) && now[0] != -2) || (!held(now[1]) && now[1] != -2)) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
 #pragma unroll
-        for (int i = 0; i < kTurns; ++i) {
-          const int live = kv - (tok0 + (i * kProducers + pw < kUnits / 2 ? 0 : kPageTokens) + piece * 16);
-          uint32_t* w = reinterpret_cast<uint32_t*>(&x[i]);
+          for (int i = 0; i < kTurns; ++i)
+            if (!held(i * kProducers + pw < kUnits / 2 ? now[0] : now[1])) x[values][i] = make_uint4(0, 0, 0, 0);
+        }
+        const int tok0 = (j0 + j) * kTileTokens;
+        if (values && tok0 + kTileTokens > kv) {                // bytes behind the end may be anything: zeros instead
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int l = live - 4 * e;
-            w[e] &= l >= 4 ? ~0u : l <= 0 ? 0u : ~0u >> (8 * (4 - l));
+          for (int i = 0; i < kTurns; ++i) {
+            const int live = kv - (tok0 + (i * kProducers + pw < kUnits / 2 ? 0 : kPageTokens) + piece * 16);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x[values][i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int l = live - 4 * e;
+              w[e] &= l >= 4 ? ~0u : l <= 0 ? 0u : ~0u >> (8 * (4 - l));
+            }
           }
         }
-      }
-      if (!values && pw == kProducers - 1 && lane < 2) {
-        const int id = lane == 0 ? now[0] : now[1];
-        const float vs = fmaxf(scales.y, 5.421010862e-20f);     // see cache_attend.cu
-        meta[j % kMeta][lane] = held(id) ? Meta{scales.x, __log2f(vs), __frcp_rn(vs), 0.f} : Meta{0.f, -INFINITY, 0.f, 0.f};   // no page: no weight
-        if (!held(id) && id != -2) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
-      }
-      mbar_wait(smem_u32(&bar_empty[slot]), ((item / C::kSlots) & 1) ^ 1, budget, &g_attend_many_status, 7);
-      __syncwarp();
-      uint8_t* dst = gen + (ring_at - base) + slot * C::kSlotBytes;
-      const bool narrow = values || D == 64;
-      // keys: rows of both pages below each other, a column block for each 64 dims; values: a column block for each page
+        if (!values && scaler) meta[j % kMeta][lane] = {scales.x, held(lane == 0 ? now[0] : now[1]) ? fmaxf(scales.y, 5.421010862e-20f) : -1.f};   // see cache_attend.cu
+        mbar_wait(smem_u32(&bar_empty[slot]), ((item / C::kSlots) & 1) ^ 1, budget, &g_attend_many_status, 7);
+        __syncwarp();
+        uint8_t* dst = gen + (ring_at - base) + slot * C::kSlotBytes;
+        const bool narrow = values || D == 64;
+        // keys: rows of both pages below each other, a column block for each 64 dims; values: a column block for each page
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const int u = i * kProducers + pw;
-        if (u >= kUnits) break;
-        uint8_t* at = dst + (narrow ? u * 1024 : (u >> 1) * 1024 + (u & 1) * (kTileTokens * 128));
-        uint4 a, b;
-        a.x = e4m3_lo(x[i].x), a.y = e4m3_hi(x[i].x), a.z = e4m3_lo(x[i].y), a.w = e4m3_hi(x[i].y);
-        b.x = e4m3_lo(x[i].z), b.y = e4m3_hi(x[i].z), b.z = e4m3_lo(x[i].w), b.w = e4m3_hi(x[i].w);
-        *reinterpret_cast<uint4*>(at + put0) = a;
-        *reinterpret_cast<uint4*>(at + put1) = b;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_full[slot]));
-      if (!values) {
-        load(true, now);
-        look_up(j + 2, later);
-      } else {
-        now[0] = next[0], now[1] = next[1], next[0] = later[0], next[1] = later[1];
+        for (int i = 0; i < kTurns; ++i) {
+          const int u = i * kProducers + pw;
+          if (u >= kUnits) break;
+          uint8_t* at = dst + (narrow ? u * 1024 : (u >> 1) * 1024 + (u & 1) * (kTileTokens * 128));
+          uint4 a, b;
+          a.x = e4m3_lo(x[values][i].x), a.y = e4m3_hi(x[values][i].x), a.z = e4m3_lo(x[values][i].y), a.w = e4m3_hi(x[values][i].y);
+          b.x = e4m3_lo(x[values][i].z), b.y = e4m3_hi(x[values][i].z), b.z = e4m3_lo(x[values][i].w), b.w = e4m3_hi(x[values][i].w);
+          *reinterpret_cast<uint4*>(at + put0) = a;
+          *reinterpret_cast<uint4*>(at + put1) = b;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_full[slot]));
         if (j + 1 < steps) {
-          load(false, now);
-          if (pw == kProducers - 1 && lane < 2) load_scales(now);
+          load(values, next, x[values]);
+          if (!values && scaler) load_scales(next);
         }
       }
+      now[0] = next[0], now[1] = next[1], next[0] = later[0], next[1] = later[1];
+      look_up(j + 3, later);
     }
     }
   }

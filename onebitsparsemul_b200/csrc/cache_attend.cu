@@ -69,12 +69,16 @@ struct FewLayout {                                // the workspace
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void load4(const uint8_t* p, uint32_t (&w)[4]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -160,7 +164,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
   int load_seq = seq;
   int64_t load_off = off + warp;
   int64_t ph = -1;                                              // (page, head) of this lane's page; -1: nothing to fetch
-  float ph_ks = 0.f, ph_lvs = 0.f, ph_ivs = 1.f;
+  float ph_ks = 0.f, ph_vs = 1.f;
   const uint32_t ring = smem_u32(smem) + warp * kRingBytes;
   auto look_up = [&](int first) {                               // pages first .. first + 31
     int s = load_seq;
@@ -178,9 +182,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
         } else {
           ph = (int64_t)id * H + head;
           ph_ks = __ldg(c.k_scale + ph);
-          const float vs = fmaxf(__ldg(c.v_scale + ph), 5.421010862e-20f);   // 2^-64: a page that nothing was stored in has scale 0
-          ph_lvs = log2f(vs);
-          ph_ivs = 1.f / vs;
+          ph_vs = __ldg(c.v_scale + ph);
         }
       }
     }
@@ -194,9 +196,6 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     if ((i & 31) == 0 && (gr & 1) == 0) look_up(i);
     const int64_t at = __shfl_sync(~0u, ph, i & 31);
     const uint32_t bar = smem_u32(&bars[warp][gr % kRing]);
-    if ((gr & 1) == 0) {
-      if (lane == (i & 31)) meta[warp][i % kMeta] = {ph_ks, ph_lvs, ph_ivs, at >= 0};
-    }
     if (lane == 0) {
       if (at >= 0) {
         mbar_expect_tx(bar, kGranule);
@@ -206,7 +205,15 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
       }
     }
   };
+  // the scales of page i, for its use; by the lane that looked them up
+  auto note_scales = [&](int i) {
+    if (i < my_pages && lane == (i & 31)) {
+      const float vs = fmaxf(ph_vs, 5.421010862e-20f);          // 2^-64: a page that nothing was stored in has scale 0
+      meta[warp][i % kMeta] = {ph_ks, log2f(vs), 1.f / vs, ph >= 0};
+    }
+  };
   for (int gr = 0; gr < kRing; ++gr) request(gr);
+  for (int i = 0; 2 * i < kRing; ++i) note_scales(i);          // behind all requests: nothing is requested later for their sake
   __syncwarp();
 
   int gr = 0;                                                   // granules used so far by this warp
@@ -288,28 +295,36 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
       __syncwarp();
       float sc[NT][4][4];
       if (md.ok) {
+        // score tile s: tokens (g / 2) 16 + 4 s + (g odd), and 2 further. The four tiles go side by side, so that no product waits
+        // for the one before it.
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {                           // 16 tokens: (g / 2) 16 + 4 s + (g odd), and 2 further
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[nt][s][i] = 0.f;
-          const uint8_t* k0 = kp + ((g >> 1) * 16 + 4 * s + (g & 1)) * D + t * 16;
+        const uint8_t* k0 = kp + ((g >> 1) * 16 + (g & 1)) * D + t * 16;
 #pragma unroll
-          for (int hf = 0; hf < D / 64; ++hf) {
-            const uint4 x = *reinterpret_cast<const uint4*>(k0 + hf * 64), y = *reinterpret_cast<const uint4*>(k0 + 2 * D + hf * 64);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int hf = 0; hf < D / 64; ++hf) {
+          uint32_t x[4][4], y[4][4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t a0 = e4m3_lo(xs[w]), a2 = e4m3_hi(xs[w]), a1 = e4m3_lo(ys[w]), a3 = e4m3_hi(ys[w]);
+          for (int s = 0; s < 4; ++s) {
+            load4(k0 + 4 * s * D + hf * 64, x[s]);
+            load4(k0 + (4 * s + 2) * D + hf * 64, y[s]);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              const uint32_t a0 = e4m3_lo(x[s][w]), a2 = e4m3_hi(x[s][w]), a1 = e4m3_lo(y[s][w]), a3 = e4m3_hi(y[s][w]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma_16816(sc[nt][s], a0, a1, a2, a3, qf[nt][hf * 4 + w][0], qf[nt][hf * 4 + w][1]);
             }
-          }
         }
       }
       __syncwarp();
       request(gr + kRing);                                      // the keys' slot is free
+      if (((gr + kRing) & 1) == 0) note_scales((gr + kRing) >> 1);
       uint32_t pf[NT][4][2];                                    // weights: B operand of k-step s
       if (md.ok) {
         bool moved = false;
@@ -384,24 +399,32 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
           }
         }
 #pragma unroll
-        for (int i = 0; i < kMT; ++i) {
-          const uint8_t* v0 = vp + (16 * i + g) * kPageTokens + t * 16;
-          const uint4 x = *reinterpret_cast<const uint4*>(v0), y = *reinterpret_cast<const uint4*>(v0 + 8 * kPageTokens);
-          uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int i0 = 0; i0 < kMT; i0 += 4) {                   // four value tiles side by side
+          uint32_t x[4][4], y[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            load4(vp + (16 * (i0 + i) + g) * kPageTokens + t * 16, x[i]);
+            load4(vp + (16 * (i0 + i) + 8 + g) * kPageTokens + t * 16, y[i]);
+          }
           if (tail) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) { xs[s] &= keep[s]; ys[s] &= keep[s]; }
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int s = 0; s < 4; ++s) { x[i][s] &= keep[s]; y[i][s] &= keep[s]; }
           }
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t a0 = e4m3_lo(xs[s]), a2 = e4m3_hi(xs[s]), a1 = e4m3_lo(ys[s]), a3 = e4m3_hi(ys[s]);
+          for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][i], a0, a1, a2, a3, pf[nt][s][0], pf[nt][s][1]);
-          }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = e4m3_lo(x[i][s]), a2 = e4m3_hi(x[i][s]), a1 = e4m3_lo(y[i][s]), a3 = e4m3_hi(y[i][s]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][i0 + i], a0, a1, a2, a3, pf[nt][s][0], pf[nt][s][1]);
+            }
         }
       }
       __syncwarp();
       request(gr + 1 + kRing);
+      if (((gr + 1 + kRing) & 1) == 0) note_scales((gr + 1 + kRing) >> 1);
       gr += 2;
       __syncwarp();
     }

@@ -22,57 +22,26 @@ import math
 
 import torch
 
-from . import _lib
-from ._lib import OneBitError
-
 __all__ = ["residual_norm", "rotary_frequencies", "rotary_tokens", "KVCache8", "CacheBatch", "cache_append", "cache_attend"]
 
 PAGE_TOKENS = 64
-_TYPES = {torch.float16: _lib.DENSE_F16, torch.bfloat16: _lib.DENSE_BF16}
-_LAYOUTS = {"half": 0, "interleaved": 1}
+_extension = None
 
 
-def _check(tensors, device):
-    """Every tensor on `device`, none of them waiting for a gradient."""
-    if device.type != "cuda":
-        raise OneBitError("no CUDA tensor: this library has no CPU path")
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"tensors on different devices: {t.device} and {device}")
-        if grad and t.requires_grad:
-            raise ValueError("a tensor wants a gradient, and this operator has none: call it under torch.no_grad()")
-
-
-def _call(fn, device, *args):
-    """fn(*args, stream) on the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
-    else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
-
-
-def _type_code(dtype):
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise TypeError(f"expected float16 or bfloat16, got {dtype}") from None
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _ext():
+    """The torch extension, whose C++ side checks the tensors and calls libonebitmul."""
+    global _extension
+    if _extension is None:
+        try:
+            import onebit_sparse_cuda
+        except ImportError as e:
+            raise ImportError("the onebit_sparse_cuda extension is missing: build it with `python -m onebitsparsemul_b200.build --all` "
+                              "(or `make torch_ext`)") from e
+        _extension = onebit_sparse_cuda
+    return _extension
 
 
 # ---- norms -------------------------------------------------------------------------------------------------------------
-
-def _rows(t, hidden):
-    """t as (rows, hidden) with contiguous rows."""
-    t = t if t.dim() == 2 else t.reshape(-1, hidden)
-    return t if t.stride(1) == 1 or hidden == 1 else t.contiguous()
-
 
 def residual_norm(x, weight, residual=None, gate=None, residual_scale=1.0, post_weight=None, eps=1e-6, out=None, residual_out=None):
     """The residual add with the norms around it, in one pass over the rows (``onebit_residual_norm``):
@@ -85,48 +54,7 @@ def residual_norm(x, weight, residual=None, gate=None, residual_scale=1.0, post_
     x's type or float32. gate: (hidden,) or x's shape, x's type. Returns (y, h), y in x's type and h in residual's; without a
     residual only y, the norm of x. `out` / `residual_out` (contiguous) receive y / h and may be x / residual themselves.
     Arithmetic and sums are float32; y is the norm of h before h's own rounding."""
-    lib = _lib.load()
-    code, dev = _type_code(x.dtype), x.device
-    _check((x, weight, residual, gate, post_weight, out, residual_out), dev)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 32768:
-        raise ValueError("x must be (..., hidden) with 1 <= hidden <= 32768")
-    hidden, shape = x.shape[-1], x.shape
-    for name, w in (("weight", weight), ("post_weight", post_weight)):
-        if w is not None and (w.dtype != x.dtype or w.shape != (hidden,)):
-            raise ValueError(f"{name} must be ({hidden},) of x's type")
-    if not (eps >= 0 and math.isfinite(eps) and math.isfinite(residual_scale)):
-        raise ValueError("eps must be finite and not negative, residual_scale finite")
-    if residual is None:
-        if gate is not None or post_weight is not None or residual_out is not None or residual_scale != 1.0:
-            raise ValueError("gate, post_weight, residual_scale and residual_out need a residual")
-    else:
-        if residual.shape != shape or residual.dtype not in (x.dtype, torch.float32):
-            raise ValueError("residual must have x's shape and x's type or float32")
-        if residual_out is None:
-            residual_out = torch.empty(shape, dtype=residual.dtype, device=dev)
-        elif residual_out.shape != shape or residual_out.dtype != residual.dtype or not residual_out.is_contiguous():
-            raise ValueError("residual_out must be contiguous with residual's shape and type")
-    gate_stride = 0
-    if gate is not None:
-        if gate.dtype != x.dtype or gate.shape not in ((hidden,), shape):
-            raise ValueError("gate must be (hidden,) or x's shape, of x's type")
-        per_row = gate.shape == shape and gate.dim() > 1
-        gate = _rows(gate, hidden) if per_row else gate.contiguous()
-        gate_stride = gate.stride(0) if per_row else 0
-    if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-    elif out.shape != shape or out.dtype != x.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous with x's shape and type")
-    x2 = _rows(x, hidden)
-    r2 = None if residual is None else _rows(residual, hidden)
-    weight = weight.contiguous()
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    rows = x2.shape[0]
-    if rows:
-        _call(lib.onebit_residual_norm, dev, x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0),
-              r2 is not None and r2.dtype == torch.float32, _ptr(gate), gate_stride, _ptr(post_weight), weight.data_ptr(),
-              out.data_ptr(), hidden, _ptr(residual_out), hidden, rows, hidden, residual_scale, eps, code)
-    return out if residual is None else (out, residual_out)
+    return _ext().residual_norm(x, weight, residual, gate, residual_scale, post_weight, eps, out, residual_out)
 
 
 # ---- rotary positions -----------------------------------------------------------------------------------------------------
@@ -168,53 +96,12 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda"):
     return f.to(device), magnitude
 
 
-def _heads(t, name, tokens=None, heads=None, dim=None):
-    if t.dim() != 3 or any(want is not None and got != want for got, want in zip(t.shape, (tokens, heads, dim))):
-        want = ", ".join("?" if w is None else str(w) for w in (tokens, heads, dim))
-        raise ValueError(f"{name} must be ({want}), got {tuple(t.shape)}")
-
-
-def _inner(t):
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
-
-
-def _rotation(inv_freq, layout, head_dim):
-    if layout not in _LAYOUTS:
-        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be a contiguous float64 vector (32 bits lose the angles of far positions)")
-    if 2 * inv_freq.numel() > head_dim:
-        raise ValueError(f"{inv_freq.numel()} pairs do not fit a head of {head_dim}")
-    return 2 * inv_freq.numel()
-
-
 def rotary_tokens(x, positions, inv_freq, layout="half", magnitude=1.0, out=None):
     """x (tokens, heads, head_dim <= 512) with the first 2 * len(inv_freq) values of every head turned by its token's position
     (``onebit_rotary``): pairs (i, i + len(inv_freq)) for "half", (2i, 2i + 1) for "interleaved"; the rest is passed on.
     positions: (tokens,) int32 or int64, any sign. inv_freq: float64, see `rotary_frequencies`. x may be a view into the rows
     of a fused projection; `out` may be x itself or any tensor of its shape with contiguous heads that does not overlap x."""
-    lib = _lib.load()
-    code, dev = _type_code(x.dtype), x.device
-    _check((x, positions, inv_freq, out), dev)
-    _heads(x, "x")
-    tokens, heads, dim = x.shape
-    if not 1 <= dim <= 512 or not 1 <= heads <= 4096 or tokens > 1 << 24:
-        raise ValueError("x must be (tokens <= 2^24, heads <= 4096, head_dim <= 512)")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,):
-        raise ValueError("positions must be (tokens,) int32 or int64")
-    rotary_dim = _rotation(inv_freq, layout, dim)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
-        raise ValueError("out must have x's shape and type and contiguous heads")
-    if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
-        raise ValueError("out overlaps x without being x")
-    x, positions = _inner(x), positions.contiguous()
-    if tokens:
-        _call(lib.onebit_rotary, dev, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-              positions.data_ptr(), positions.dtype == torch.int64, inv_freq.data_ptr(), rotary_dim, _LAYOUTS[layout], magnitude,
-              tokens, heads, dim, code)
-    return out
+    return _ext().rotary_tokens(x, positions, inv_freq, layout, magnitude, out)
 
 
 # ---- the cache ----------------------------------------------------------------------------------------------------------------
@@ -223,23 +110,11 @@ class KVCache8:
     """The tensors of an 8-bit key/value cache (layout in the module's docstring), checked once here. Bytes that no append
     has written must be finite codes (`empty` makes zeros); a page may be given to another sequence at any time."""
 
-    __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "pages", "kv_heads", "head_dim", "device")
+    __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "pages", "kv_heads", "head_dim")
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
-        if k_pages.dim() != 4 or k_pages.shape[2] != PAGE_TOKENS or k_pages.shape[3] not in (64, 128):
-            raise ValueError("k_pages must be (pages, kv_heads, 64, 64 or 128)")
-        pages, heads, _, dim = k_pages.shape
-        if v_pages.shape != (pages, heads, dim, PAGE_TOKENS) or k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
-            raise ValueError(f"with {pages} pages of {heads} heads of {dim}: v_pages must be ({pages}, {heads}, {dim}, 64), scales ({pages}, {heads})")
-        if k_pages.dtype != torch.float8_e4m3fn or v_pages.dtype != torch.float8_e4m3fn or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
-            raise TypeError("pages must be float8_e4m3fn, scales float32")
-        for t in (k_pages, v_pages, k_scale, v_scale):
-            if not t.is_contiguous() or t.device != k_pages.device:
-                raise ValueError("pages and scales must be contiguous, on one device")
-        if pages < 1 or not 1 <= heads <= 4096:
-            raise ValueError("need at least one page and 1 to 4096 heads")
+        self.pages, self.kv_heads, self.head_dim = _ext().check_cache(k_pages, v_pages, k_scale, v_scale)
         self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
-        self.pages, self.kv_heads, self.head_dim, self.device = pages, heads, dim, k_pages.device
 
     @classmethod
     def empty(cls, pages, kv_heads, head_dim, device="cuda"):
@@ -274,24 +149,13 @@ class CacheBatch:
     values stay on the device and may be rewritten between steps (a captured step reads them anew). A page number or a range
     that lies outside its tensor is left out, and ``onebit_check_device_status`` reports it."""
 
-    __slots__ = ("q_start", "kv_len", "block_table", "max_new", "seqs", "width", "device")
+    __slots__ = ("q_start", "kv_len", "block_table", "max_new", "seqs", "width")
 
     def __init__(self, q_start, kv_len, block_table, max_new=None):
-        if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or block_table.dtype != torch.int32:
-            raise TypeError("q_start, kv_len and block_table must be int32")
-        if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1 or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-            raise ValueError("block_table must be (sequences, width), at least 1 x 1, with contiguous rows")
-        seqs, width = block_table.shape
-        if q_start.shape != (seqs + 1,) or kv_len.shape != (seqs,) or not q_start.is_contiguous() or not kv_len.is_contiguous():
-            raise ValueError(f"with {seqs} sequences: q_start must be ({seqs + 1},), kv_len ({seqs},), both contiguous")
-        if q_start.device != block_table.device or kv_len.device != block_table.device:
-            raise ValueError("q_start, kv_len and block_table must be on one device")
-        if seqs > 1 << 16 or width > 1 << 24:
-            raise ValueError("at most 2^16 sequences of 2^24 pages")
         if max_new is not None and max_new < 1:
             raise ValueError("max_new must be positive")
-        self.q_start, self.kv_len, self.block_table = q_start, kv_len, block_table
-        self.max_new, self.seqs, self.width, self.device = max_new or 0, seqs, width, block_table.device
+        self.seqs, self.width = _ext().check_batch(q_start, kv_len, block_table)
+        self.q_start, self.kv_len, self.block_table, self.max_new = q_start, kv_len, block_table, max_new or 0
 
 
 def cache_append(k, v, cache, batch, q=None, inv_freq=None, layout="half", magnitude=1.0, q_out=None):
@@ -304,52 +168,8 @@ def cache_append(k, v, cache, batch, q=None, inv_freq=None, layout="half", magni
     stored as the largest value of the page's scale. A NaN key stays NaN; a token with a NaN value has it stored as 0 and its key
     made NaN, so that the queries that see the token answer NaN and no others. A page that a step writes must belong to one
     sequence of the batch only."""
-    lib = _lib.load()
-    code, dev = _type_code(k.dtype), k.device
-    _check((k, v, q, inv_freq, q_out), dev)
-    if cache.device != dev or batch.device != dev:
-        raise ValueError("cache, batch and tensors must be on one device")
-    tokens, H, D = k.shape[0], cache.kv_heads, cache.head_dim
-    _heads(k, "k", tokens, H, D)
-    _heads(v, "v", tokens, H, D)
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
-        raise TypeError("q, k and v must have one type")
-    if tokens > 1 << 24:
-        raise ValueError("at most 2^24 tokens")
-    rotary_dim = 0 if inv_freq is None else _rotation(inv_freq, layout, D)
-    heads = H
-    if q is not None:
-        _heads(q, "q", tokens, None, D)
-        heads = q.shape[1]
-        if inv_freq is None:
-            raise ValueError("q is only turned: it needs inv_freq")
-        if heads % H or not 1 <= heads <= 4096:
-            raise ValueError(f"{heads} query heads are no multiple of {H} cache heads")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
-            raise ValueError("q_out must have q's shape and type and contiguous heads")
-        if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
-            raise ValueError("q_out overlaps q without being q")
-        q = _inner(q)
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    k, v = _inner(k), _inner(v)
-    if tokens:
-        qs, os_ = ((0, 0), (0, 0)) if q is None else (q.stride(), q_out.stride())
-        ks, vs = k.stride(), v.stride()
-        _call(lib.onebit_cache_append, dev, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _ptr(q), qs[0], qs[1], _ptr(q_out), os_[0], os_[1],
-              _ptr(inv_freq), rotary_dim, _LAYOUTS.get(layout, 0), magnitude, cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
-              cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.pages, batch.q_start.data_ptr(), batch.kv_len.data_ptr(),
-              batch.block_table.data_ptr(), batch.block_table.stride(0), batch.width, tokens, batch.seqs, heads, H, D, code)
-    return q_out
-
-
-def _aligned(t):
-    """t with 16-byte aligned heads, copied if it has none."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return _ext().cache_append(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, batch.q_start, batch.kv_len, batch.block_table,
+                               q, inv_freq, layout, magnitude, q_out)
 
 
 def cache_attend(q, cache, batch, scale=None, causal=True, out=None):
@@ -358,31 +178,5 @@ def cache_attend(q, cache, batch, scale=None, causal=True, out=None):
     h // (heads // kv_heads). causal: a token sees the positions up to its own (the new tokens are the last ones of the
     sequence), else the whole sequence. scale: head_dim ** -0.5 by default. A row that sees nothing is zero. `out`: contiguous,
     q's shape and type."""
-    lib = _lib.load()
-    code, dev = _type_code(q.dtype), q.device
-    _check((q, out), dev)
-    if cache.device != dev or batch.device != dev:
-        raise ValueError("cache, batch and tensors must be on one device")
-    _heads(q, "q", None, None, cache.head_dim)
-    tokens, heads, D = q.shape
-    if heads % cache.kv_heads or not 1 <= heads <= 4096:
-        raise ValueError(f"{heads} query heads are no multiple of {cache.kv_heads} cache heads")
-    if tokens > 1 << 24:
-        raise ValueError("at most 2^24 tokens")
-    scale = D ** -0.5 if scale is None else scale
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError("out must be contiguous (and 16-byte aligned) with q's shape and type")
-    if tokens:
-        q = _aligned(q)
-        qs = q.stride()
-        need = lib.onebit_cache_attend_workspace(batch.width, tokens, batch.seqs, heads, cache.kv_heads, D, batch.max_new)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _call(lib.onebit_cache_attend, dev, q.data_ptr(), qs[0], qs[1], out.data_ptr(), heads * D, D, cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
-              cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.pages, batch.q_start.data_ptr(), batch.kv_len.data_ptr(),
-              batch.block_table.data_ptr(), batch.block_table.stride(0), batch.width, tokens, batch.seqs, heads, cache.kv_heads, D,
-              batch.max_new, scale, causal, code, _ptr(ws), need)
-    return out
+    return _ext().cache_attend(q, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, batch.q_start, batch.kv_len, batch.block_table,
+                               batch.max_new, scale, causal, out)

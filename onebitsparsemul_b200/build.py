@@ -14,6 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libonebitmul.so")
 SOURCES = ["api.cu", "pack.cu", "mask.cu", "relayout.cu", "gemm_simple.cu", "gemm_decode.cu", "gemm_decode_sm100.cu", "gemm_prefill_sm100.cu", "gemm_prefill2_sm100.cu", "gemm_prefill3_sm100.cu", "gemm_prefill_splitk_sm100.cu", "noalloc.cu", "host_pipeline.cu",
            "norm.cu", "rotary_append.cu", "cache_attend.cu", "cache_attend_sm100.cu"]
+EXTENSION_SOURCES = ["torch_kernel_cuda.cpp", "torch_block_ops.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
@@ -70,19 +71,23 @@ def build_torch_extension(force: bool = False) -> str:
 
     lib = build_library()
     root = os.path.dirname(HERE)
-    src = os.path.join(CSRC, "torch_kernel_cuda.cpp")
+    srcs = [os.path.join(CSRC, f) for f in EXTENSION_SOURCES]
     out = os.path.join(root, "onebit_sparse_cuda" + sysconfig.get_config_var("EXT_SUFFIX"))
     hdr = os.path.join(root, "include", "onebit_sparse_tensor.h")
-    if not force and not _stale(out, [src, hdr, lib]):
+    objdir = os.path.join(HERE, "build")
+    objs = [os.path.join(objdir, f.replace(".cpp", ".o")) for f in EXTENSION_SOURCES]
+    if not force and not _stale(out, [*srcs, hdr, lib]):
         return out
     inc = [f"-I{p}" for p in cpp_extension.include_paths("cuda")] + [f"-I{sysconfig.get_paths()['include']}",
                                                                   f"-I{os.path.join(root, 'include')}"]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *inc, src, "-o", out, f"-L{HERE}", "-lonebitmul", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-           "-lc10", "-lc10_cuda", "-ltorch_cuda", f"-Wl,-rpath,$ORIGIN/{os.path.basename(HERE)}", f"-Wl,-rpath,{torch_lib}"]
-    subprocess.check_call(cmd)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc]
+    procs = [subprocess.Popen(["g++", *flags, "-c", src, "-o", obj]) for src, obj in zip(srcs, objs) if force or _stale(obj, [src, hdr])]
+    if any([p.wait() for p in procs]):
+        raise RuntimeError("g++ failed for onebit_sparse_cuda")
+    subprocess.check_call(["g++", "-shared", *objs, "-o", out, f"-L{HERE}", "-lonebitmul", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+                           "-lc10", "-lc10_cuda", "-ltorch_cuda", f"-Wl,-rpath,$ORIGIN/{os.path.basename(HERE)}", f"-Wl,-rpath,{torch_lib}"])
     return out
 
 

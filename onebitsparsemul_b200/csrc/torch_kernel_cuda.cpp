@@ -51,7 +51,10 @@ void onebit_mul_impl(const torch::Tensor& A, const torch::Tensor& B, const torch
 
 }  // namespace
 
+void bind_block_ops(pybind11::module_& m);   // torch_block_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("onebit_mul", &onebit_mul_impl, "C = onebit 2:4 sparse A x fp16 B", pybind11::arg("A"), pybind11::arg("B"),
         pybind11::arg("meta_or_C"), pybind11::arg("C_or_meta"), pybind11::arg("scale") = c10::optional<torch::Tensor>());
+  bind_block_ops(m);
 }

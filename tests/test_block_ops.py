@@ -10,9 +10,9 @@ from onebitsparsemul_b200 import _lib, build
 from tests import block_plain as plain
 
 
-@pytest.fixture(scope="module")
+@pytest.fixture(scope="module", autouse=True)
 def lib():
-    build.build_library()
+    build.build_torch_extension()
     return _lib.load()
 
 

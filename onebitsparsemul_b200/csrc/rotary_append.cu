@@ -65,6 +65,7 @@ struct AppendArgs {
 constexpr int kRotTokens = 4;          // tokens per CTA
 constexpr int kRotThreads = 256;
 constexpr int kMaxHalf = 256;
+constexpr int kBatch = 4;              // pieces that a thread has under way
 
 // pair i of the head at p: values a, b at offsets (oa, ob)
 __device__ __forceinline__ void pair_at(const Rotation& r, int i, int& oa, int& ob) {
@@ -72,74 +73,104 @@ __device__ __forceinline__ void pair_at(const Rotation& r, int i, int& oa, int& 
   ob = r.interleaved ? 2 * i + 1 : i + r.half;
 }
 
-// The heads of up to kRotTokens tokens, from the table of their cos and sin in shared memory. W = 8: rotation and pass-through
-// in pieces of 8 values.
-template <typename T, int W>
+// The heads of up to kRotTokens tokens, from the table of their cos and sin in shared memory. A head is cut into pieces, a thread
+// keeps its piece and goes from head to head. W = 8: pieces of 8 values (the rotated ones of "half" with their partners), kBatch
+// of them loaded before the first is stored; in place, a piece is read and written by its own thread only.
+template <typename T, int W, int THREADS>
 __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n, const float2 (&cs)[kRotTokens][kMaxHalf], const bool (&skip)[kRotTokens]) {
   const Rotation& r = a.rot;
-  const bool in_place = a.x == a.y;
-  // units of a head: W pairs each (half) or W / 2 pairs (interleaved), then the pass-through in pieces of W
   const int pairs_per = W == 1 ? 1 : (r.interleaved ? W / 2 : W);
   const int turning = r.half / pairs_per;
-  const int passing = in_place ? 0 : (a.head_dim - 2 * r.half) / W;
+  const int passing = a.x == a.y ? 0 : (a.head_dim - 2 * r.half) / W;
   const int per_head = turning + passing;
-  const int total = n * a.heads * per_head;
-  for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int piece = u % per_head, th = u / per_head;
-    const int head = th % a.heads, tt = th / a.heads;
-    if (skip[tt]) continue;
-    const T* x = static_cast<const T*>(a.x) + (int64_t)(t0 + tt) * a.x_ts + (int64_t)head * a.x_hs;
-    T* y = static_cast<T*>(a.y) + (int64_t)(t0 + tt) * a.y_ts + (int64_t)head * a.y_hs;
-    if (piece >= turning) {
-      const int o = 2 * r.half + (piece - turning) * W;
-      if constexpr (W == 8) *reinterpret_cast<uint4*>(y + o) = *reinterpret_cast<const uint4*>(x + o);
-      else y[o] = x[o];
-      continue;
-    }
-    if constexpr (W == 1) {
+  if (per_head == 0) return;
+  if constexpr (W == 1) {
+    for (int u = threadIdx.x; u < n * a.heads * per_head; u += THREADS) {
+      const int piece = u % per_head, th = u / per_head, head = th % a.heads, tt = th / a.heads;
+      if (skip[tt]) continue;
+      const T* x = static_cast<const T*>(a.x) + (int64_t)(t0 + tt) * a.x_ts + (int64_t)head * a.x_hs;
+      T* y = static_cast<T*>(a.y) + (int64_t)(t0 + tt) * a.y_ts + (int64_t)head * a.y_hs;
+      if (piece >= turning) {
+        y[2 * r.half + piece - turning] = x[2 * r.half + piece - turning];
+        continue;
+      }
       int oa, ob;
       pair_at(r, piece, oa, ob);
       const float2 c = cs[tt][piece];
       const float va = to_f32(x[oa]), vb = to_f32(x[ob]);
       y[oa] = from_f32<T>(va * c.x - vb * c.y);
       y[ob] = from_f32<T>(vb * c.x + va * c.y);
-    } else if (r.interleaved) {
-      float v[8];
-      load8(x + piece * 8, v);
+    }
+  } else {
+    const int rows = max(1, THREADS / per_head);               // heads that the CTA takes at once
+    const bool one = per_head > THREADS;                       // never with head_dim <= 512: at most 64 pieces
+    const int piece = threadIdx.x % per_head;
+    if (one || (int)threadIdx.x >= rows * per_head) return;
+    int head = threadIdx.x / per_head, tt = 0;
+    while (head >= a.heads) { head -= a.heads; ++tt; }
+    const bool turn = piece < turning, pairs = turn && !r.interleaved;
+    const int o0 = turn ? piece * 8 : 2 * r.half + (piece - turning) * 8;
+    while (tt < n) {
+      uint4 va[kBatch], vb[kBatch];
+      int64_t at[kBatch];
+      int tok[kBatch];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 c = cs[tt][piece * 4 + i];
-        const float va = v[2 * i], vb = v[2 * i + 1];
-        v[2 * i] = va * c.x - vb * c.y;
-        v[2 * i + 1] = vb * c.x + va * c.y;
+      for (int i = 0; i < kBatch; ++i) {
+        tok[i] = tt < n && !skip[tt] ? tt : -1;
+        at[i] = (int64_t)(t0 + tt) * a.y_ts + (int64_t)head * a.y_hs + o0;
+        if (tok[i] >= 0) {
+          const T* x = static_cast<const T*>(a.x) + (int64_t)(t0 + tt) * a.x_ts + (int64_t)head * a.x_hs + o0;
+          va[i] = *reinterpret_cast<const uint4*>(x);
+          if (pairs) vb[i] = *reinterpret_cast<const uint4*>(x + r.half);
+        }
+        head += rows;
+        while (head >= a.heads) { head -= a.heads; ++tt; }
       }
-      store8(y + piece * 8, v);
-    } else {
-      float va[8], vb[8];
-      load8(x + piece * 8, va);
-      load8(x + r.half + piece * 8, vb);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 c = cs[tt][piece * 8 + i];
-        const float p = va[i], q = vb[i];
-        va[i] = p * c.x - q * c.y;
-        vb[i] = q * c.x + p * c.y;
+      for (int i = 0; i < kBatch; ++i) {
+        if (tok[i] < 0) continue;
+        T* y = static_cast<T*>(a.y) + at[i];
+        if (!turn) {
+          *reinterpret_cast<uint4*>(y) = va[i];
+        } else if (r.interleaved) {
+          const float4* c4 = reinterpret_cast<const float4*>(&cs[tok[i]][piece * 4]);       // cos, sin of two pairs
+          const uint32_t w[4] = {va[i].x, va[i].y, va[i].z, va[i].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 c = c4[e / 2];
+            const float2 v = unpack2(w[e], T{});
+            const float cc = e & 1 ? c.z : c.x, ss = e & 1 ? c.w : c.y;
+            o[e] = pack2(v.x * cc - v.y * ss, v.y * cc + v.x * ss, T{});
+          }
+          *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+          const float4* c4 = reinterpret_cast<const float4*>(&cs[tok[i]][piece * 8]);
+          const uint32_t w[4] = {va[i].x, va[i].y, va[i].z, va[i].w}, z[4] = {vb[i].x, vb[i].y, vb[i].z, vb[i].w};
+          uint32_t o[4], q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 c = c4[e];
+            const float2 v = unpack2(w[e], T{}), u = unpack2(z[e], T{});
+            o[e] = pack2(v.x * c.x - u.x * c.y, v.y * c.z - u.y * c.w, T{});
+            q[e] = pack2(u.x * c.x + v.x * c.y, u.y * c.z + v.y * c.w, T{});
+          }
+          *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(y + r.half) = make_uint4(q[0], q[1], q[2], q[3]);
+        }
       }
-      store8(y + piece * 8, va);
-      store8(y + r.half + piece * 8, vb);
     }
   }
 }
 
+template <int THREADS>
 __device__ __forceinline__ void fill_cos_sin(const Rotation& r, const int64_t (&pos)[kRotTokens], int n, float2 (&cs)[kRotTokens][kMaxHalf]) {
-  for (int u = threadIdx.x; u < n * r.half; u += kRotThreads) {
-    const int i = u % r.half, tt = u / r.half;
-    cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), pos[tt], r.magnitude);
-  }
+  for (int i = threadIdx.x % 64; i < r.half; i += 64)          // 64 pairs of each of THREADS / 64 tokens at a time
+    for (int tt = threadIdx.x / 64; tt < n; tt += THREADS / 64) cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), pos[tt], r.magnitude);
 }
 
 template <typename T, int W> __global__ void __launch_bounds__(kRotThreads) ob_rotary_kernel(const RotaryArgs a) {
-  __shared__ float2 cs[kRotTokens][kMaxHalf];
+  __shared__ __align__(16) float2 cs[kRotTokens][kMaxHalf];
   __shared__ int64_t pos[kRotTokens];
   __shared__ bool skip[kRotTokens];
   const int t0 = blockIdx.x * kRotTokens, n = min(kRotTokens, a.tokens - t0);
@@ -149,26 +180,44 @@ template <typename T, int W> __global__ void __launch_bounds__(kRotThreads) ob_r
     skip[threadIdx.x] = false;
   }
   __syncthreads();
-  fill_cos_sin(a.rot, pos, n, cs);
+  fill_cos_sin<kRotThreads>(a.rot, pos, n, cs);
   __syncthreads();
-  rotate_tokens<T, W>(a, t0, n, cs, skip);
+  rotate_tokens<T, W, kRotThreads>(a, t0, n, cs, skip);
 }
 
 // Number of sequences s with key(s) <= x, counted by the whole CTA (keys do not decrease with s).
-template <typename F> __device__ __forceinline__ int count_not_above(int seqs, int x, F key) {
+template <int THREADS, typename F> __device__ __forceinline__ int count_not_above(int seqs, int x, F key) {
   int c = 0;
-  for (int s0 = 0; s0 < seqs; s0 += kRotThreads) {
+  for (int s0 = 0; s0 < seqs; s0 += THREADS) {
     const int s = s0 + threadIdx.x;
     c += __syncthreads_count(s < seqs && key(s) <= x);
   }
   return c;
 }
 
+__device__ __forceinline__ float finite_max(float m, float v) {
+  v = fabsf(v);
+  return v <= 3.402823466e38f ? fmaxf(m, v) : m;
+}
 
+// the largest value of the CTA's threads
+template <int THREADS> __device__ __forceinline__ float cta_max(float v, float (&red)[THREADS / 32]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) v = fmaxf(v, red[w]);
+  return v;
+}
+
+// 2 D threads: 16 groups of 4 tokens (a word of the transposed values) x D / 8 groups of 8 values. Bound by the queries' bytes on
+// prompts and by its chain of dependent loads (batch, page, tokens) on single tokens; at 64 registers four CTAs share an SM.
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(kRotThreads) ob_cache_append_kernel(const AppendArgs a, const RotaryArgs q) {
-  __shared__ float2 cs[kPageTokens][D / 2];
-  __shared__ float red[2][kRotThreads / 32];
+__global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(const AppendArgs a, const RotaryArgs q) {
+  constexpr int kThreads = 2 * D;
+  __shared__ __align__(16) float2 cs[kPageTokens][D / 2];
+  __shared__ float red[2][kThreads / 32];
   __shared__ int nan_token[kPageTokens];
   const int tid = threadIdx.x;
   const BatchArgs& b = a.b;
@@ -180,182 +229,218 @@ __global__ void __launch_bounds__(kRotThreads) ob_cache_append_kernel(const Appe
     __shared__ int64_t pos[kRotTokens];
     __shared__ bool skip[kRotTokens];
     const int t0 = ((int)blockIdx.x - a.page_slots * a.kv_heads) * kRotTokens, n = min(kRotTokens, q.tokens - t0);
-    for (int tt = 0; tt < n; ++tt) {
-      const int t = t0 + tt;
-      const int c = count_not_above(b.seqs + 1, t, [&](int s) { return b.q_start[s]; });   // sequence c - 1 holds token t
-      if (tid == 0) {
-        skip[tt] = c < 1 || c > b.seqs;                       // before the first or behind the last sequence
-        pos[tt] = 0;
-        if (!skip[tt]) pos[tt] = (int64_t)b.kv_len[c - 1] - b.q_start[c] + t;
-      }
+    int c[kRotTokens] = {};                                    // sequence c - 1 holds the token
+    for (int s0 = 0; s0 <= b.seqs; s0 += kThreads) {
+      const int s = s0 + tid, start = s <= b.seqs ? b.q_start[s] : 0x7fffffff;
+#pragma unroll
+      for (int tt = 0; tt < kRotTokens; ++tt) c[tt] += __syncthreads_count(start <= t0 + tt);
     }
+#pragma unroll
+    for (int tt = 0; tt < kRotTokens; ++tt)
+      if (tid == tt && tt < n) {
+        skip[tt] = c[tt] < 1 || c[tt] > b.seqs;                // before the first or behind the last sequence
+        pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c[tt] - 1] - b.q_start[c[tt]] + t0 + tt;
+      }
     __syncthreads();
-    fill_cos_sin(q.rot, pos, n, qcs);
+    fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
     __syncthreads();
-    rotate_tokens<T, W>(q, t0, n, qcs, skip);
+    rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip);
     return;
   }
 
-  // ---- a page of one head ----
-  // Page slots: sequence s owns slots [floor(q_start[s] / 64) + 2 s, floor(q_start[s+1] / 64) + 2 (s + 1)), at least as many as
-  // n tokens can touch pages.
+  // ---- pages of one head ----
+  // Sequence s owns the slots [floor(q_start[s] / 64) + s, floor(q_start[s+1] / 64) + s + 1): at least floor(n / 64) + 1. n tokens
+  // touch at most one page more than that, which the first slot then takes too.
   const int head = (int)blockIdx.x % a.kv_heads, slot = (int)blockIdx.x / a.kv_heads;
-  auto first_slot = [&](int s) { return b.q_start[s] / kPageTokens + 2 * s; };
-  const int seq = count_not_above(b.seqs, slot, first_slot) - 1;
+  auto first_slot = [&](int s) { return b.q_start[s] / kPageTokens + s; };
+  const int seq = count_not_above<kThreads>(b.seqs, slot, first_slot) - 1;
   if (seq < 0) return;
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
   if (n <= 0 || kv <= 0) return;
-  const int before = kv - n;                                  // may be negative: the first -before tokens have no place
-  const int block = max(before, 0) / kPageTokens + slot - first_slot(seq);
-  const int base = block * kPageTokens;
-  if (block < 0 || base >= kv) return;                        // block < 0: q_start runs backwards
-  const int page = block < b.table_width ? b.table[(int64_t)seq * b.table_stride + block] : -1;
-  if (q0 < 0 || q1 > a.tokens || page < 0 || page >= a.pages) {
+  if (q0 < 0 || q1 > a.tokens) {
     if (tid == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
     return;
   }
-  const int lo = max(before - base, 0), hi = min(kv - base, kPageTokens);      // places of the new tokens in the page
-  const bool fresh = before <= base;
-  const int64_t row0 = (int64_t)q0 + base - before;           // row of the token at place 0 (negative if that one is older)
+  const int before = kv - n;                                  // may be negative: the first -before tokens have no place
+  const int mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + seq + 1 - (q0 / kPageTokens + seq);
+  if (mine < 0) return;                                       // q_start runs backwards
   const Rotation& r = a.rot;
-
-  if (tid < kPageTokens) nan_token[tid] = 0;
-  for (int u = tid; u < (hi - lo) * r.half; u += kRotThreads) {
-    const int i = u % r.half, tt = lo + u / r.half;
-    cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), (int64_t)base + tt, r.magnitude);
-  }
-  __syncthreads();
-
-  // thread = 4 tokens (one word of the transposed values) x 8 values; a warp = 8 x 4 of those
   constexpr int kVecs = D / 8;
-  constexpr int kUsed = 16 * kVecs;                           // 256 threads at D = 128, 128 at D = 64
-  const int quad = (tid & 7) + 8 * ((tid >> 5) / (kVecs / 4));
+  const int quad = (tid & 7) + 8 * ((tid >> 5) / (kVecs / 4)); // a warp: 8 x 4 of the groups
   const int vec = ((tid >> 3) & 3) + 4 * ((tid >> 5) % (kVecs / 4));
-  const bool mine = tid < kUsed;
   const int d0 = vec * 8;
-  float kf[4][8], vf[4][8];
-  float k_max = 0.f, v_max = 0.f;
-  auto finite_max = [](float m, float v) { v = fabsf(v); return v <= 3.402823466e38f ? fmaxf(m, v) : m; };
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int place = quad * 4 + i;
-    if (!mine || place < lo || place >= hi) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kf[i][e] = vf[i][e] = 0.f;
+
+  for (int64_t block = max(before, 0) / kPageTokens + mine; block * kPageTokens < kv; block += slots) {
+    const int base = (int)block * kPageTokens;
+    const int page = block < b.table_width ? b.table[(int64_t)seq * b.table_stride + block] : -1;
+    if (page < 0 || page >= a.pages) {
+      if (tid == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
       continue;
     }
-    const T* kr = static_cast<const T*>(a.k) + (row0 + place) * a.k_ts + (int64_t)head * a.k_hs;
-    const T* vr = static_cast<const T*>(a.v) + (row0 + place) * a.v_ts + (int64_t)head * a.v_hs;
+    const int lo = max(before - base, 0), hi = min(kv - base, kPageTokens);      // places of the new tokens in the page
+    const bool fresh = before <= base;
+    const int64_t row0 = (int64_t)q0 + base - before;         // row of the token at place 0 (negative if that one is older)
+    const int64_t ph = (int64_t)page * a.kv_heads + head;
+    const float k_old = fresh ? 0.f : a.k_scale[ph], v_old = fresh ? 0.f : a.v_scale[ph];
+
+    // values first: raw words of four tokens; keys are on their way meanwhile
+    uint4 vr[4], kr[4];
     if constexpr (W == 8) {
-      load8(kr + d0, kf[i]);
-      load8(vr + d0, vf[i]);
-      if (d0 < 2 * r.half) {
-        if (r.interleaved) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 c = cs[place][d0 / 2 + e];
-            const float x = kf[i][2 * e], y = kf[i][2 * e + 1];
-            kf[i][2 * e] = x * c.x - y * c.y;
-            kf[i][2 * e + 1] = y * c.x + x * c.y;
-          }
-        } else {
-          float other[8];
-          const bool first = d0 < r.half;
-          const int p0 = first ? d0 : d0 - r.half;
-          load8(kr + (first ? d0 + r.half : p0), other);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 c = cs[place][p0 + e];
-            kf[i][e] = first ? kf[i][e] * c.x - other[e] * c.y : kf[i][e] * c.x + other[e] * c.y;
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int place = quad * 4 + i;
+        const bool in = place >= lo && place < hi;
+        vr[i] = in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + (row0 + place) * a.v_ts + (int64_t)head * a.v_hs + d0) : make_uint4(0, 0, 0, 0);
+        kr[i] = in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + (row0 + place) * a.k_ts + (int64_t)head * a.k_hs + d0) : make_uint4(0, 0, 0, 0);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = d0 + e;
-        kf[i][e] = to_f32(kr[d]);
-        vf[i][e] = to_f32(vr[d]);
-        if (d < 2 * r.half) {
-          const int p = r.interleaved ? d / 2 : (d < r.half ? d : d - r.half);
-          const bool first = r.interleaved ? (d & 1) == 0 : d < r.half;
-          const float2 c = cs[place][p];
-          const float other = to_f32(kr[r.interleaved ? d ^ 1 : (first ? d + r.half : d - r.half)]);
-          kf[i][e] = first ? kf[i][e] * c.x - other * c.y : kf[i][e] * c.x + other * c.y;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int place = quad * 4 + i;
+        const bool in = place >= lo && place < hi;
+        const T* v = static_cast<const T*>(a.v) + (row0 + place) * a.v_ts + (int64_t)head * a.v_hs + d0;
+        const T* k = static_cast<const T*>(a.k) + (row0 + place) * a.k_ts + (int64_t)head * a.k_hs + d0;
+        uint32_t wv[4] = {}, wk[4] = {};
+        if (in)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            wv[e] = pack2(to_f32(v[2 * e]), to_f32(v[2 * e + 1]), T{});
+            wk[e] = pack2(to_f32(k[2 * e]), to_f32(k[2 * e + 1]), T{});
+          }
+        vr[i] = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+        kr[i] = make_uint4(wk[0], wk[1], wk[2], wk[3]);
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      k_max = finite_max(k_max, kf[i][e]);
-      v_max = finite_max(v_max, vf[i][e]);
-      if (isnan(vf[i][e])) { vf[i][e] = 0.f; nan_token[place] = 1; }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    k_max = fmaxf(k_max, __shfl_xor_sync(~0u, k_max, o));
-    v_max = fmaxf(v_max, __shfl_xor_sync(~0u, v_max, o));
-  }
-  if ((tid & 31) == 0) { red[0][tid >> 5] = k_max; red[1][tid >> 5] = v_max; }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kRotThreads / 32; ++w) { k_max = fmaxf(k_max, red[0][w]); v_max = fmaxf(v_max, red[1][w]); }
+    if (tid < kPageTokens) nan_token[tid] = 0;
+    for (int i = tid % (D / 2); i < r.half; i += D / 2)       // D / 2 pairs of 4 tokens at a time
+      for (int tt = lo + tid / (D / 2); tt < hi; tt += 4) cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), (int64_t)base + tt, r.magnitude);
+    __syncthreads();
 
-  const int64_t ph = (int64_t)page * a.kv_heads + head;
-  float k_s = scale_for(k_max), v_s = scale_for(v_max), k_ratio = 1.f, v_ratio = 1.f;
-  if (!fresh) {
-    const float k_old = a.k_scale[ph], v_old = a.v_scale[ph];
-    k_s = fmaxf(k_s, k_old);
-    v_s = fmaxf(v_s, v_old);
-    k_ratio = k_old / k_s;
-    v_ratio = v_old / v_s;
-  }
-  __syncthreads();                                            // every thread has read the old scales
-  if (tid == 0) { a.k_scale[ph] = k_s; a.v_scale[ph] = v_s; }
-  if (!mine) return;
-  const float k_inv = 1.f / k_s, v_inv = 1.f / v_s;           // exact: powers of two
-
-  // keys: 8 bytes of each token
-  uint8_t* kp = a.k_pages + ph * (kPageTokens * D) + d0;
+    float v_max = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int place = quad * 4 + i;
-    const bool is_new = place >= lo && place < hi;
-    if (!is_new && !(fresh || (place < lo && k_ratio != 1.f))) continue;
-    uint2* at = reinterpret_cast<uint2*>(kp + place * D);
-    uint8_t c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (is_new) {
+    for (int i = 0; i < 4; ++i) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&vr[i]);
+      bool nan = false;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = to_e4m3(kf[i][e] * k_inv);
-      if (d0 == 0 && nan_token[place]) c[0] = 0x7F;
-    } else if (place < lo) {
-      const uint2 old = *at;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = to_e4m3(from_e4m3((uint8_t)((e < 4 ? old.x : old.y) >> (8 * (e & 3)))) * k_ratio);
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2(w[e], T{});
+        v_max = finite_max(finite_max(v_max, f.x), f.y);
+        if (isnan(f.x)) { w[e] &= 0xFFFF0000u; nan = true; }  // stored as 0
+        if (isnan(f.y)) { w[e] &= 0x0000FFFFu; nan = true; }
+      }
+      if (nan) nan_token[quad * 4 + i] = 1;
     }
-    *at = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | (uint32_t)c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | (uint32_t)c[7] << 24);
-  }
-  // values: 4 tokens of each of 8 rows
-  const bool any_new = quad * 4 < hi && quad * 4 + 4 > lo;
-  const bool any_old = quad * 4 < lo;
-  if (!any_new && !fresh && !(any_old && v_ratio != 1.f)) return;
-  const bool whole = fresh || (quad * 4 >= lo && quad * 4 + 4 <= hi);
-  uint8_t* vp = a.v_pages + ph * (kPageTokens * D) + quad * 4;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    uint32_t* at = reinterpret_cast<uint32_t*>(vp + (d0 + e) * kPageTokens);
-    const uint32_t old = whole ? 0u : *at;
-    uint32_t w = 0;
+    // keys, turned
+    float kf[4][8], k_max = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int place = quad * 4 + i;
-      uint8_t c = (uint8_t)(old >> (8 * i));
-      if (place >= lo && place < hi) c = to_e4m3(vf[i][e] * v_inv);
-      else if (place < lo && v_ratio != 1.f) c = to_e4m3(from_e4m3(c) * v_ratio);
-      w |= (uint32_t)c << (8 * i);
+      const uint32_t w[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2(w[e], T{});
+        kf[i][2 * e] = f.x, kf[i][2 * e + 1] = f.y;
+      }
+      if (place >= lo && place < hi && d0 < 2 * r.half) {
+        const T* k = static_cast<const T*>(a.k) + (row0 + place) * a.k_ts + (int64_t)head * a.k_hs;
+        if constexpr (W == 8) {
+          if (r.interleaved) {
+            const float4* c4 = reinterpret_cast<const float4*>(&cs[place][d0 / 2]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 c = c4[e / 2];
+              const float cc = e & 1 ? c.z : c.x, ss = e & 1 ? c.w : c.y, x = kf[i][2 * e], y = kf[i][2 * e + 1];
+              kf[i][2 * e] = x * cc - y * ss;
+              kf[i][2 * e + 1] = y * cc + x * ss;
+            }
+          } else {
+            const bool front = d0 < r.half;
+            const int p0 = front ? d0 : d0 - r.half;
+            float other[8];
+            load8(k + (front ? d0 + r.half : p0), other);     // a neighbour's piece: from the first-level cache
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 c = cs[place][p0 + e];
+              kf[i][e] = front ? kf[i][e] * c.x - other[e] * c.y : kf[i][e] * c.x + other[e] * c.y;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int d = d0 + e;
+            if (d < 2 * r.half) {
+              const int p = r.interleaved ? d / 2 : (d < r.half ? d : d - r.half);
+              const bool front = r.interleaved ? (d & 1) == 0 : d < r.half;
+              const float2 c = cs[place][p];
+              const float other = to_f32(k[r.interleaved ? d ^ 1 : (front ? d + r.half : d - r.half)]);
+              kf[i][e] = front ? kf[i][e] * c.x - other * c.y : kf[i][e] * c.x + other * c.y;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k_max = finite_max(k_max, kf[i][e]);
     }
-    *at = w;
+    v_max = cta_max<kThreads>(v_max, red[0]);
+    k_max = cta_max<kThreads>(k_max, red[1]);                 // both CTA barriers: every thread has read the old scales
+    float k_s = scale_for(k_max), v_s = scale_for(v_max), k_ratio = 1.f, v_ratio = 1.f;
+    if (!fresh) {
+      k_s = fmaxf(k_s, k_old);
+      v_s = fmaxf(v_s, v_old);
+      k_ratio = k_old / k_s;
+      v_ratio = v_old / v_s;
+    }
+    if (tid == 0) { a.k_scale[ph] = k_s; a.v_scale[ph] = v_s; }
+    const float k_inv = 1.f / k_s, v_inv = 1.f / v_s;         // exact: powers of two
+
+    // keys: 8 bytes of each token
+    uint8_t* kp = a.k_pages + ph * (kPageTokens * D) + d0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int place = quad * 4 + i;
+      const bool is_new = place >= lo && place < hi;
+      if (!is_new && !(fresh || (place < lo && k_ratio != 1.f))) continue;
+      uint2* at = reinterpret_cast<uint2*>(kp + place * D);
+      uint32_t c[2] = {0, 0};
+      if (is_new) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e / 4] |= (uint32_t)to_e4m3(kf[i][e] * k_inv) << (8 * (e & 3));
+        if (d0 == 0 && nan_token[place]) c[0] = (c[0] & ~0xFFu) | 0x7Fu;
+      } else if (place < lo) {
+        const uint2 old = *at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          c[e / 4] |= (uint32_t)to_e4m3(from_e4m3((uint8_t)((e < 4 ? old.x : old.y) >> (8 * (e & 3)))) * k_ratio) << (8 * (e & 3));
+      }
+      *at = make_uint2(c[0], c[1]);
+    }
+    // values: 4 tokens of each of 8 rows
+    const bool any_new = quad * 4 < hi && quad * 4 + 4 > lo;
+    if (any_new || fresh || (quad * 4 < lo && v_ratio != 1.f)) {
+      const bool whole = fresh || (quad * 4 >= lo && quad * 4 + 4 <= hi);
+      uint8_t* vp = a.v_pages + ph * (kPageTokens * D) + quad * 4;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(vp + (d0 + e) * kPageTokens);
+        const uint32_t old = whole ? 0u : *at;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int place = quad * 4 + i;
+          uint8_t code = (uint8_t)(old >> (8 * i));
+          if (place >= lo && place < hi) {
+            const uint32_t half = reinterpret_cast<const uint32_t*>(&vr[i])[e / 2];
+            const float2 f = unpack2(half, T{});
+            code = to_e4m3((e & 1 ? f.y : f.x) * v_inv);
+          } else if (place < lo && v_ratio != 1.f) {
+            code = to_e4m3(from_e4m3(code) * v_ratio);
+          }
+          w |= (uint32_t)code << (8 * i);
+        }
+        *at = w;
+      }
+    }
+    __syncthreads();                                          // the next page's tables go over this one's
   }
 }
 
@@ -393,13 +478,13 @@ cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream) {
   a.b = {c.q_start, c.kv_len, c.table, c.table_stride, (int)c.table_width, (int)c.seqs};
   a.rot = {c.inv_freq, c.rotary_dim / 2, c.interleaved, c.magnitude};
   a.tokens = (int)c.tokens;
-  a.page_slots = (int)(c.tokens / kPageTokens + 2 * c.seqs);
+  a.page_slots = (int)(c.tokens / kPageTokens + c.seqs);
   RotaryArgs q{c.q, c.q_out, c.q_ts, c.q_hs, c.qo_ts, c.qo_hs, nullptr, 0, c.q ? (int)c.tokens : 0, (int)c.heads, (int)c.head_dim, a.rot};
   const bool wide = wide_rotation(c.rotary_dim, c.interleaved) && wide_rows(c.k, c.k_ts, c.k_hs) && wide_rows(c.v, c.v_ts, c.v_hs) &&
                     wide_rows(c.q, c.q_ts, c.q_hs) && wide_rows(c.q_out, c.qo_ts, c.qo_hs);
   const int64_t blocks = (int64_t)a.page_slots * a.kv_heads + (q.tokens + kRotTokens - 1) / kRotTokens;
   auto go = [&](auto t, auto d, auto w) {
-    ob_cache_append_kernel<decltype(t), decltype(d)::value, decltype(w)::value><<<(unsigned)blocks, kRotThreads, 0, stream>>>(a, q);
+    ob_cache_append_kernel<decltype(t), decltype(d)::value, decltype(w)::value><<<(unsigned)blocks, 2 * decltype(d)::value, 0, stream>>>(a, q);
     return cudaGetLastError();
   };
   auto by_width = [&](auto t, auto d) {

@@ -94,4 +94,22 @@ __device__ __forceinline__ float scale_for(float amax) {
   return ldexpf(1.f, min(max(e, kMinScaleExp), kMaxScaleExp));
 }
 
+// ---- programmatic dependent launch -----------------------------------------------------------------------------------------
+// A decode step is a chain of kernels of a few microseconds. They are launched so that a grid may start while its
+// predecessor drains, and each waits here, before its first access to memory, until the predecessor is complete.
+__device__ __forceinline__ void follow_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_following(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace ob_block

@@ -110,11 +110,11 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
   const int group = (int)(c.heads / c.kv_heads);
   const int H = (int)c.kv_heads;
   long long budget = 2000000000ll;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (lane == 0)
     for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  follow_previous_kernel();
 
   // ---- this CTA's piece: every thread sums a run of sequences, the CTA scans the sums ----
   const int run = (int)((c.seqs + kWarps * 32 - 1) / (kWarps * 32));
@@ -496,7 +496,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
 template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_combine_kernel(const ob::CacheAttendCall c, const FewLayout ws, int rows) {
   constexpr int kPitch = D + 4;
   __shared__ float red[8], total[8], part[8][D];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  follow_previous_kernel();
   const Header h = ws.headers[blockIdx.x];
   if (h.last < 0) return;
   const int group = (int)(c.heads / c.kv_heads);
@@ -555,16 +555,9 @@ template <typename T, int D, int NT> cudaError_t launch_few(const ob::CacheAtten
   FewLayout ws{static_cast<Header*>(workspace), reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((grid * sizeof(Header) + 255) & ~size_t(255)))};
   cudaError_t e = cudaFuncSetAttribute(ob_attend_few_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  ob_attend_few_kernel<T, D, NT><<<grid, kWarps * 32, smem, stream>>>(c, ws);
-  e = cudaGetLastError();
+  e = launch_following(ob_attend_few_kernel<T, D, NT>, dim3(grid), kWarps * 32, smem, stream, c, ws);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, 8 * NT), cfg.blockDim = dim3(256), cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, ob_attend_combine_kernel<T, D>, c, ws, 8 * NT);
+  return launch_following(ob_attend_combine_kernel<T, D>, dim3(grid, 8 * NT), 256, 0, stream, c, ws, 8 * NT);
 }
 
 }  // namespace

@@ -35,11 +35,37 @@ template <bool WARP_ROW> __device__ __forceinline__ float row_sum(float v, float
   return v;
 }
 
+// W values as they lie in memory
+template <typename T, int W> struct Raw {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void zero() { v = from_f32<T>(0.f); }
+  __device__ __forceinline__ void values(float (&f)[W]) const { f[0] = to_f32(v); }
+};
+template <typename T> struct Raw<T, 8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 x = unpack2(w[i], T{}); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
+  }
+};
+template <> struct Raw<float, 8> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void values(float (&f)[8]) const { f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w; }
+};
+
 // V chunks of W values per thread; chunk j of thread t starts at value (j * threads_of_row + t) * W. W = 8: 16-byte accesses
-// (hidden % 8 == 0 and every row aligned); W = 1: any width and alignment.
+// (hidden % 8 == 0 and every row aligned); W = 1: any width and alignment. Bound by memory on many rows: what a row is read into
+// stays packed until its sum is there, so that few registers a thread let enough rows be under way on an SM.
 template <typename T, typename R, int V, int W, bool WARP_ROW>
 __global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a) {
   __shared__ float scratch[2][32];
+  follow_previous_kernel();
   const int tpr = WARP_ROW ? 32 : blockDim.x;
   const int t = WARP_ROW ? (threadIdx.x & 31) : threadIdx.x;
   const int64_t row = WARP_ROW ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -53,83 +79,84 @@ __global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a
   R* hout = res ? static_cast<R*>(a.h) + row * a.h_stride : nullptr;
   const float inv_n = 1.f / (float)a.hidden;
 
-  float u[V][W], r[V][W];
+  Raw<T, W> xr[V];
+  Raw<R, W> rr[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int c = (j * tpr + t) * W;
-    const bool in = c < a.hidden;
-    if constexpr (W == 8) {
-      if (in) { load8(x + c, u[j]); if (res) load8(res + c, r[j]); }
-      else for (int i = 0; i < W; ++i) u[j][i] = r[j][i] = 0.f;
-    } else {
-      u[j][0] = in ? to_f32(x[c]) : 0.f;
-      r[j][0] = in && res ? to_f32(res[c]) : 0.f;
+    xr[j].zero();
+    rr[j].zero();
+    if (c < a.hidden) {
+      xr[j].load(x + c);
+      if (res) rr[j].load(res + c);
     }
   }
-  if (res) {
-    float f = 1.f;
-    if (post) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < W; ++i) s += u[j][i] * u[j][i];
-      f = rsqrtf(row_sum<WARP_ROW>(s, scratch[0]) * inv_n + a.eps);
-    }
+  float f = 1.f;
+  if (post) {
+    float s = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * tpr + t) * W;
-      if (c >= a.hidden) continue;
-      float p[W], g[W];
-      if constexpr (W == 8) {
-        if (post) load8(post + c, p);
-        if (gate) load8(gate + c, g);
-      } else {
-        if (post) p[0] = to_f32(post[c]);
-        if (gate) g[0] = to_f32(gate[c]);
-      }
+      float u[W];
+      xr[j].values(u);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float v = u[j][i];
-        if (post) v *= f * p[i];
-        if (gate) v *= g[i];
-        u[j][i] = r[j][i] + a.residual_scale * v;
-      }
-      if constexpr (W == 8) store8(hout + c, u[j]);
-      else hout[c] = from_f32<R>(u[j][0]);
+      for (int i = 0; i < W; ++i) s += u[i] * u[i];
     }
+    f = rsqrtf(row_sum<WARP_ROW>(s, scratch[0]) * inv_n + a.eps);
   }
-  float s = 0.f;
+  float h[V][W], s = 0.f;
 #pragma unroll
-  for (int j = 0; j < V; ++j)
+  for (int j = 0; j < V; ++j) {
+    const int c = (j * tpr + t) * W;
+    xr[j].values(h[j]);
+    if (res && c < a.hidden) {
+      float r[W];
+      rr[j].values(r);
+      if (post) {
+        Raw<T, W> p;
+        p.load(post + c);
+        float v[W];
+        p.values(v);
 #pragma unroll
-    for (int i = 0; i < W; ++i) s += u[j][i] * u[j][i];
-  const float f = rsqrtf(row_sum<WARP_ROW>(s, scratch[1]) * inv_n + a.eps);
+        for (int i = 0; i < W; ++i) h[j][i] *= f * v[i];
+      }
+      if (gate) {
+        Raw<T, W> g;
+        g.load(gate + c);
+        float v[W];
+        g.values(v);
+#pragma unroll
+        for (int i = 0; i < W; ++i) h[j][i] *= v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) h[j][i] = r[i] + a.residual_scale * h[j][i];
+      if constexpr (W == 8) store8(hout + c, h[j]);
+      else hout[c] = from_f32<R>(h[j][0]);
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += h[j][i] * h[j][i];
+  }
+  f = rsqrtf(row_sum<WARP_ROW>(s, scratch[1]) * inv_n + a.eps);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int c = (j * tpr + t) * W;
     if (c >= a.hidden) continue;
-    if constexpr (W == 8) {
-      float w[8];
-      load8(weight + c, w);
+    Raw<T, W> w;
+    w.load(weight + c);
+    float v[W];
+    w.values(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] *= u[j][i] * f;
-      store8(y + c, w);
-    } else {
-      y[c] = from_f32<T>(u[j][0] * f * to_f32(weight[c]));
-    }
+    for (int i = 0; i < W; ++i) v[i] *= h[j][i] * f;
+    if constexpr (W == 8) store8(y + c, v);
+    else y[c] = from_f32<T>(v[0]);
   }
 }
 
 template <typename T, typename R, int V, int W>
 cudaError_t launch_rows(const NormArgs& a, int threads, cudaStream_t stream) {
-  if (threads == 32) {
-    constexpr int kRows = 4;                                  // rows (warps) per CTA
-    ob_residual_norm_kernel<T, R, V, W, true><<<(unsigned)((a.rows + kRows - 1) / kRows), 32 * kRows, 0, stream>>>(a);
-  } else {
-    ob_residual_norm_kernel<T, R, V, W, false><<<(unsigned)a.rows, threads, 0, stream>>>(a);
-  }
-  return cudaGetLastError();
+  constexpr int kRows = 4;                                    // rows (warps) per CTA where a warp has a row
+  if (threads == 32)
+    return launch_following(ob_residual_norm_kernel<T, R, V, W, true>, dim3((unsigned)((a.rows + kRows - 1) / kRows)), 32 * kRows, 0, stream, a);
+  return launch_following(ob_residual_norm_kernel<T, R, V, W, false>, dim3((unsigned)a.rows), threads, 0, stream, a);
 }
 
 template <typename T, typename R> cudaError_t launch_types(const NormArgs& a, bool wide, cudaStream_t stream) {

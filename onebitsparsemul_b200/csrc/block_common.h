@@ -71,11 +71,12 @@ __device__ __forceinline__ uint64_t turns_per_position(double angular_frequency)
   t -= floor(t);
   return __double2ull_rz(t * 18446744073709551616.0);
 }
+// cos and sin (times magnitude) by the special function unit: the angle lies in [-pi, pi), where its results are within 2^-21.2
+// of the exact ones, a thousandth of the 16-bit types' rounding; sincospif would be several times the instructions of the rest.
 __device__ __forceinline__ float2 cos_sin(uint64_t per_position, int64_t position, float magnitude) {
   const uint64_t phase = per_position * (uint64_t)position;
-  float s, c;
-  sincospif((float)(int32_t)(uint32_t)(phase >> 32) * 4.656612873077393e-10f /* 2^-31: half turns in [-1, 1) */, &s, &c);
-  return make_float2(c * magnitude, s * magnitude);
+  const float angle = (float)(int32_t)(uint32_t)(phase >> 32) * 1.4629180792671596e-9f;      // pi * 2^-31
+  return make_float2(__cosf(angle) * magnitude, __sinf(angle) * magnitude);
 }
 
 // ---- e4m3 -----------------------------------------------------------------------------------------------------------------

@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a
 template <typename T, typename R, int V, int W>
 cudaError_t launch_rows(const NormArgs& a, int threads, cudaStream_t stream) {
   constexpr int kRows = 4;                                    // rows (warps) per CTA where a warp has a row
-  if (threads == 32)
-    return launch_following(ob_residual_norm_kernel<T, R, V, W, true>, dim3((unsigned)((a.rows + kRows - 1) / kRows)), 32 * kRows, 0, stream, a);
+  if constexpr (V * W <= 16)                                  // the only chunkings that a warp alone can be given
+    if (threads == 32)
+      return launch_following(ob_residual_norm_kernel<T, R, V, W, true>, dim3((unsigned)((a.rows + kRows - 1) / kRows)), 32 * kRows, 0, stream, a);
   return launch_following(ob_residual_norm_kernel<T, R, V, W, false>, dim3((unsigned)a.rows), threads, 0, stream, a);
 }
 

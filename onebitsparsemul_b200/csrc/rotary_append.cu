@@ -62,7 +62,7 @@ struct AppendArgs {
   int page_slots;                      // CTAs of the append half of the grid: page slots x kv_heads
 };
 
-constexpr int kRotTokens = 4;          // tokens per CTA
+constexpr int kAppendTokens = 2, kFewTokens = 4;   // query tokens per CTA of an append: with prompts, with steps
 constexpr int kRotThreads = 256;
 constexpr int kMaxHalf = 256;
 constexpr int kBatch = 4;              // pieces that a thread has under way
@@ -73,18 +73,20 @@ __device__ __forceinline__ void pair_at(const Rotation& r, int i, int& oa, int& 
   ob = r.interleaved ? 2 * i + 1 : i + r.half;
 }
 
-// The heads of up to kRotTokens tokens, from the table of their cos and sin in shared memory. A head is cut into pieces, a thread
+// The heads of up to TOKENS tokens, from the table of their cos and sin in shared memory. A head is cut into pieces, a thread
 // keeps its piece and goes from head to head. W = 8: pieces of 8 values (the rotated ones of "half" with their partners), kBatch
-// of them loaded before the first is stored; in place, a piece is read and written by its own thread only.
-template <typename T, int W, int THREADS>
-__device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n, const float2 (&cs)[kRotTokens][kMaxHalf], const bool (&skip)[kRotTokens]) {
+// of them loaded before the first is stored; in place, a piece is read and written by its own thread only. make_table() (all
+// threads; ends with a barrier) fills cs and skip while the first pieces are on their way.
+template <typename T, int W, int THREADS, int TOKENS, typename F>
+__device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n, const float2 (&cs)[TOKENS][kMaxHalf], const bool (&skip)[TOKENS], F make_table) {
   const Rotation& r = a.rot;
   const int pairs_per = W == 1 ? 1 : (r.interleaved ? W / 2 : W);
   const int turning = r.half / pairs_per;
   const int passing = a.x == a.y ? 0 : (a.head_dim - 2 * r.half) / W;
   const int per_head = turning + passing;
-  if (per_head == 0) return;
+  if (per_head == 0) return;                                   // nothing is turned and the rest is there already
   if constexpr (W == 1) {
+    make_table();
     for (int u = threadIdx.x; u < n * a.heads * per_head; u += THREADS) {
       const int piece = u % per_head, th = u / per_head, head = th % a.heads, tt = th / a.heads;
       if (skip[tt]) continue;
@@ -102,23 +104,21 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n
       y[ob] = from_f32<T>(vb * c.x + va * c.y);
     }
   } else {
-    const int rows = max(1, THREADS / per_head);               // heads that the CTA takes at once
-    const bool one = per_head > THREADS;                       // never with head_dim <= 512: at most 64 pieces
+    const int rows = THREADS / per_head;                       // heads that the CTA takes at once; a head has at most 64 pieces
     const int piece = threadIdx.x % per_head;
-    if (one || (int)threadIdx.x >= rows * per_head) return;
-    int head = threadIdx.x / per_head, tt = 0;
+    int head = threadIdx.x / per_head, tt = head < rows ? 0 : n;   // threads left over take none
     while (head >= a.heads) { head -= a.heads; ++tt; }
     const bool turn = piece < turning, pairs = turn && !r.interleaved;
     const int o0 = turn ? piece * 8 : 2 * r.half + (piece - turning) * 8;
-    while (tt < n) {
+    for (bool first = true; first || tt < n; first = false) {
       uint4 va[kBatch], vb[kBatch];
       int64_t at[kBatch];
       int tok[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        tok[i] = tt < n && !skip[tt] ? tt : -1;
+        tok[i] = tt < n ? tt : -1;
         at[i] = (int64_t)(t0 + tt) * a.y_ts + (int64_t)head * a.y_hs + o0;
-        if (tok[i] >= 0) {
+        if (tt < n) {
           const T* x = static_cast<const T*>(a.x) + (int64_t)(t0 + tt) * a.x_ts + (int64_t)head * a.x_hs + o0;
           va[i] = *reinterpret_cast<const uint4*>(x);
           if (pairs) vb[i] = *reinterpret_cast<const uint4*>(x + r.half);
@@ -126,9 +126,10 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n
         head += rows;
         while (head >= a.heads) { head -= a.heads; ++tt; }
       }
+      if (first) make_table();
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (tok[i] < 0) continue;
+        if (tok[i] < 0 || skip[tok[i]]) continue;
         T* y = static_cast<T*>(a.y) + at[i];
         if (!turn) {
           *reinterpret_cast<uint4*>(y) = va[i];
@@ -163,27 +164,28 @@ __device__ __forceinline__ void rotate_tokens(const RotaryArgs& a, int t0, int n
   }
 }
 
-template <int THREADS>
-__device__ __forceinline__ void fill_cos_sin(const Rotation& r, const int64_t (&pos)[kRotTokens], int n, float2 (&cs)[kRotTokens][kMaxHalf]) {
+template <int THREADS, int TOKENS>
+__device__ __forceinline__ void fill_cos_sin(const Rotation& r, const int64_t (&pos)[TOKENS], int n, float2 (&cs)[TOKENS][kMaxHalf]) {
   for (int i = threadIdx.x % 64; i < r.half; i += 64)          // 64 pairs of each of THREADS / 64 tokens at a time
     for (int tt = threadIdx.x / 64; tt < n; tt += THREADS / 64) cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), pos[tt], r.magnitude);
 }
 
-template <typename T, int W> __global__ void __launch_bounds__(kRotThreads) ob_rotary_kernel(const RotaryArgs a) {
+template <typename T, int W, int TOKENS> __global__ void __launch_bounds__(kRotThreads, 4) ob_rotary_kernel(const RotaryArgs a) {
   follow_previous_kernel();
-  __shared__ __align__(16) float2 cs[kRotTokens][kMaxHalf];
-  __shared__ int64_t pos[kRotTokens];
-  __shared__ bool skip[kRotTokens];
-  const int t0 = blockIdx.x * kRotTokens, n = min(kRotTokens, a.tokens - t0);
-  if (threadIdx.x < n) {
-    pos[threadIdx.x] = a.positions_i64 ? static_cast<const int64_t*>(a.positions)[t0 + threadIdx.x]
-                                       : (int64_t) static_cast<const int*>(a.positions)[t0 + threadIdx.x];
-    skip[threadIdx.x] = false;
-  }
-  __syncthreads();
-  fill_cos_sin<kRotThreads>(a.rot, pos, n, cs);
-  __syncthreads();
-  rotate_tokens<T, W, kRotThreads>(a, t0, n, cs, skip);
+  __shared__ __align__(16) float2 cs[TOKENS][kMaxHalf];
+  __shared__ int64_t pos[TOKENS];
+  __shared__ bool skip[TOKENS];
+  const int t0 = blockIdx.x * TOKENS, n = min(TOKENS, a.tokens - t0);
+  rotate_tokens<T, W, kRotThreads>(a, t0, n, cs, skip, [&] {
+    if (threadIdx.x < n) {
+      pos[threadIdx.x] = a.positions_i64 ? static_cast<const int64_t*>(a.positions)[t0 + threadIdx.x]
+                                         : (int64_t) static_cast<const int*>(a.positions)[t0 + threadIdx.x];
+      skip[threadIdx.x] = false;
+    }
+    __syncthreads();
+    fill_cos_sin<kRotThreads>(a.rot, pos, n, cs);
+    __syncthreads();
+  });
 }
 
 // Number of sequences s with key(s) <= x, counted by the whole CTA (keys do not decrease with s).
@@ -224,29 +226,32 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
   const int tid = threadIdx.x;
   const BatchArgs& b = a.b;
 
-  if ((int)blockIdx.x >= a.page_slots * a.kv_heads) {
-    // ---- queries: up to kRotTokens tokens ----
-    auto& qcs = reinterpret_cast<float2(&)[kRotTokens][kMaxHalf]>(cs);
-    static_assert(sizeof(cs) >= sizeof(float2) * kRotTokens * kMaxHalf, "the queries' table lies in the keys'");
-    __shared__ int64_t pos[kRotTokens];
-    __shared__ bool skip[kRotTokens];
-    const int t0 = ((int)blockIdx.x - a.page_slots * a.kv_heads) * kRotTokens, n = min(kRotTokens, q.tokens - t0);
-    int c[kRotTokens] = {};                                    // sequence c - 1 holds the token
-    for (int s0 = 0; s0 <= b.seqs; s0 += kThreads) {
-      const int s = s0 + tid, start = s <= b.seqs ? b.q_start[s] : 0x7fffffff;
+  // the CTAs of pages come first: they are the longer ones
+  const int items = a.page_slots * a.kv_heads;
+  if ((int)blockIdx.x >= items) {
+    // ---- queries: up to kAppendTokens tokens ----
+    auto& qcs = reinterpret_cast<float2(&)[kAppendTokens][kMaxHalf]>(cs);
+    static_assert(sizeof(cs) >= sizeof(float2) * kAppendTokens * kMaxHalf, "the queries' table lies in the keys'");
+    __shared__ int64_t pos[kAppendTokens];
+    __shared__ bool skip[kAppendTokens];
+    const int t0 = ((int)blockIdx.x - items) * kAppendTokens, n = min(kAppendTokens, q.tokens - t0);
+    rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip, [&] {
+      int c[kAppendTokens] = {};                                 // sequence c - 1 holds the token
+      for (int s0 = 0; s0 <= b.seqs; s0 += kThreads) {
+        const int s = s0 + tid, start = s <= b.seqs ? b.q_start[s] : 0x7fffffff;
 #pragma unroll
-      for (int tt = 0; tt < kRotTokens; ++tt) c[tt] += __syncthreads_count(start <= t0 + tt);
-    }
-#pragma unroll
-    for (int tt = 0; tt < kRotTokens; ++tt)
-      if (tid == tt && tt < n) {
-        skip[tt] = c[tt] < 1 || c[tt] > b.seqs;                // before the first or behind the last sequence
-        pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c[tt] - 1] - b.q_start[c[tt]] + t0 + tt;
+        for (int tt = 0; tt < kAppendTokens; ++tt) c[tt] += __syncthreads_count(start <= t0 + tt);
       }
-    __syncthreads();
-    fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
-    __syncthreads();
-    rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip);
+#pragma unroll
+      for (int tt = 0; tt < kAppendTokens; ++tt)
+        if (tid == tt && tt < n) {
+          skip[tt] = c[tt] < 1 || c[tt] > b.seqs;             // before the first or behind the last sequence
+          pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c[tt] - 1] - b.q_start[c[tt]] + t0 + tt;
+        }
+      __syncthreads();
+      fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
+      __syncthreads();
+    });
     return;
   }
 
@@ -453,9 +458,9 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
 template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_cache_append_few_kernel(const AppendArgs a, const RotaryArgs q) {
   follow_previous_kernel();
   constexpr int kThreads = 128;
-  __shared__ __align__(16) float2 qcs[kRotTokens][kMaxHalf];
-  __shared__ int64_t pos[kRotTokens];
-  __shared__ bool skip[kRotTokens];
+  __shared__ __align__(16) float2 qcs[kFewTokens][kMaxHalf];
+  __shared__ int64_t pos[kFewTokens];
+  __shared__ bool skip[kFewTokens];
   const int lane = threadIdx.x & 31;
   const BatchArgs& b = a.b;
   const int page_ctas = (a.page_slots * a.kv_heads + 3) / 4;
@@ -466,18 +471,19 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
     return c;
   };
   if ((int)blockIdx.x >= page_ctas) {
-    const int t0 = ((int)blockIdx.x - page_ctas) * kRotTokens, n = min(kRotTokens, q.tokens - t0);
-    const int tt = threadIdx.x >> 5;                          // a warp finds a token's sequence
-    static_assert(kRotTokens == kThreads / 32, "a token per warp");
-    const int c = count(b.seqs + 1, t0 + tt, [&](int s) { return b.q_start[s]; });
-    if (lane == 0) {
-      skip[tt] = c < 1 || c > b.seqs;
-      pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c - 1] - b.q_start[c] + t0 + tt;
-    }
-    __syncthreads();
-    fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
-    __syncthreads();
-    rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip);
+    const int t0 = ((int)blockIdx.x - page_ctas) * kFewTokens, n = min(kFewTokens, q.tokens - t0);
+    static_assert(kFewTokens == kThreads / 32, "a token per warp");
+    rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip, [&] {
+      const int tt = threadIdx.x >> 5;                        // a warp finds a token's sequence
+      const int c = count(b.seqs + 1, t0 + tt, [&](int s) { return b.q_start[s]; });
+      if (lane == 0) {
+        skip[tt] = c < 1 || c > b.seqs;
+        pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c - 1] - b.q_start[c] + t0 + tt;
+      }
+      __syncthreads();
+      fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
+      __syncthreads();
+    });
     return;
   }
 
@@ -581,9 +587,15 @@ cudaError_t launch_rotary(const void* x, int64_t x_ts, int64_t x_hs, void* y, in
   const RotaryArgs a{x, y, x_ts, x_hs, y_ts, y_hs, positions, positions_i64, (int)tokens, (int)heads, (int)head_dim,
                      {inv_freq, rotary_dim / 2, interleaved, magnitude}};
   const bool wide = head_dim % 8 == 0 && wide_rotation(rotary_dim, interleaved) && wide_rows(x, x_ts, x_hs) && wide_rows(y, y_ts, y_hs);
-  const unsigned grid = (unsigned)((tokens + kRotTokens - 1) / kRotTokens);
-  if (bf16) return launch_following(wide ? ob_rotary_kernel<__nv_bfloat16, 8> : ob_rotary_kernel<__nv_bfloat16, 1>, dim3(grid), kRotThreads, 0, stream, a);
-  return launch_following(wide ? ob_rotary_kernel<__half, 8> : ob_rotary_kernel<__half, 1>, dim3(grid), kRotThreads, 0, stream, a);
+  // tokens per CTA: two where latency counts, eight (one table for all, more under way) on many. 32 heads of 128, 4096 tokens:
+  // 18.1 us with two, 15.9 with eight; 20 heads, 37 tokens: 2.7 and 5.0
+  auto go = [&](auto t, auto per) {
+    constexpr int kTokens = decltype(per)::value;
+    using T = decltype(t);
+    return launch_following(wide ? ob_rotary_kernel<T, 8, kTokens> : ob_rotary_kernel<T, 1, kTokens>, dim3((unsigned)((tokens + kTokens - 1) / kTokens)), kRotThreads, 0, stream, a);
+  };
+  auto by_count = [&](auto t) { return tokens <= 1024 ? go(t, std::integral_constant<int, 2>{}) : go(t, std::integral_constant<int, 8>{}); };
+  return bf16 ? by_count(__nv_bfloat16{}) : by_count(__half{});
 }
 
 cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream) {
@@ -598,11 +610,11 @@ cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream) {
   RotaryArgs q{c.q, c.q_out, c.q_ts, c.q_hs, c.qo_ts, c.qo_hs, nullptr, 0, c.q ? (int)c.tokens : 0, (int)c.heads, (int)c.head_dim, a.rot};
   const bool wide = wide_rotation(c.rotary_dim, c.interleaved) && wide_rows(c.k, c.k_ts, c.k_hs) && wide_rows(c.v, c.v_ts, c.v_hs) &&
                     wide_rows(c.q, c.q_ts, c.q_hs) && wide_rows(c.q_out, c.qo_ts, c.qo_hs);
-  const int64_t items = (int64_t)a.page_slots * a.kv_heads, q_ctas = (q.tokens + kRotTokens - 1) / kRotTokens;
+  const int64_t items = (int64_t)a.page_slots * a.kv_heads;
   // Few tokens a sequence on average: a warp's rolled loops. Measured for 64 sequences of 1 / 2 / 4 / 8 tokens, 8 heads of 128
   // with 32 query heads: 6.2 / 9.2 / 15.4 / 27.8 us, against 13.4 / 14.1 / 12.5 / 15.3 us.
   const bool few = c.tokens <= 2 * c.seqs;
-  const int64_t blocks = (few ? (items + 3) / 4 : items) + q_ctas;
+  const int64_t blocks = few ? (items + 3) / 4 + (q.tokens + kFewTokens - 1) / kFewTokens : items + (q.tokens + kAppendTokens - 1) / kAppendTokens;
   auto go = [&](auto t, auto d, auto w) {
     constexpr int kDim = decltype(d)::value, kWidth = decltype(w)::value;
     using T = decltype(t);

@@ -491,3 +491,89 @@ def test_prompt_and_single_steps_agree(dtype):
                 out, spread, delta, least, _ = plain.attend(q, plain.Cache(cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale), batch.q_start, batch.kv_len, table, dim ** -0.5, True)
                 assert ((got.cpu().double() - out).abs() <= plain.attend_tolerance(out, spread, delta, least, dtype)).all()
     assert status_ok()
+
+
+def small_stack(**kw):
+    from onebitsparsemul_b200.decode_loop import CachedLlamaStack
+    model = CachedLlamaStack(blocks=2, hidden=256, intermediate=512, heads=4, kv_heads=2, head_dim=64, device=DEV, seed=3, **kw)
+    for b in model.blocks:
+        b.input_norm.copy_(1 + 0.1 * gen(1)(256))
+        b.post_norm.copy_(1 + 0.1 * gen(2)(256))
+    assert ob.replace_linear_layers(model) == 8
+    return model
+
+
+def test_cached_stack_block_by_block():
+    """The packed stack's forward, operator by operator: each output against the plain form of the operator on its own inputs."""
+    model = small_stack(rotary=dict(base=5000.0, scaling=("linear", 2.0), layout="interleaved"))
+    from onebitsparsemul_b200.decode_loop import CachedDecoder
+    dec = CachedDecoder(model, 3, 200)
+    new = [70, 1, 33]
+    x = gen(4)(sum(new), 256).to(F16)
+    seen = []
+    keep = {}
+    from onebitsparsemul_b200 import block_ops
+
+    def spy(name):
+        real = keep[name] = getattr(block_ops, name)
+
+        def call(*args, **kw):
+            before = [a.clone() if torch.is_tensor(a) else a for a in args]
+            kb = {k: v.clone() if torch.is_tensor(v) else v for k, v in kw.items()}
+            cache = plain.Cache(args[2].k_pages, args[2].v_pages, args[2].k_scale, args[2].v_scale) if name == "cache_append" else None
+            got = real(*args, **kw)
+            seen.append((name, before, kb, [t.clone() if torch.is_tensor(t) else t for t in (got if isinstance(got, tuple) else (got,))], cache, args))
+            return got
+        setattr(block_ops, name, call)
+
+    for n in ("residual_norm", "cache_append", "cache_attend"):
+        spy(n)
+    try:
+        y = dec.prompt(x, new).clone()
+    finally:
+        for n, real in keep.items():
+            setattr(block_ops, n, real)
+    assert [s[0] for s in seen] == ["residual_norm"] + ["cache_append", "cache_attend", "residual_norm", "residual_norm"] * 2
+    pos = torch.cat([torch.arange(n) for n in new])
+    for name, args, kw, got, cache, live in seen:
+        if name == "residual_norm":
+            check_norm(got[0], got[1] if len(got) > 1 else None, args[0], args[1], kw.get("residual"), None, 1.0, None, kw["eps"])
+        elif name == "cache_append":
+            check_rotary(got[0], kw["q"], pos, kw["inv_freq"], "interleaved")
+        else:
+            c, b = live[1], live[2]
+            want = plain.Cache(c.k_pages, c.v_pages, c.k_scale, c.v_scale)
+            out, spread, delta, least, _ = plain.attend(args[0], want, b.q_start, b.kv_len, b.block_table, 0.125, True)
+            assert ((got[0].cpu().double() - out).abs() <= plain.attend_tolerance(out, spread, delta, least, F16)).all()
+    assert torch.equal(y, seen[-1][3][0]) and status_ok()
+
+
+def test_cached_decoder_prompts_then_graphed_steps():
+    """Prompts, graphed steps, another ragged prompt and more steps: the same numbers as the model called eagerly on a cache of
+    its own, and refusals when a sequence is full."""
+    from onebitsparsemul_b200.decode_loop import CachedDecoder
+    model = small_stack()
+    a, b = CachedDecoder(model, 3, 150), CachedDecoder(model, 3, 150)
+    n = gen(6)
+
+    def eager(x):
+        b._grow([1] * 3)
+        b.kv_len.add_(1)
+        with torch.no_grad():
+            return model(x, b.caches, b.step_batch)
+
+    for lengths, steps in (([5, 64, 20], 40), ([30, 0, 3], 5), ([0, 0, 0], 2)):
+        x = n(sum(lengths), 256).to(F16)
+        assert torch.equal(a.prompt(x, lengths), b.prompt(x, lengths))
+        for _ in range(steps):
+            x = n(3, 256).to(F16)
+            assert torch.equal(a.step(x), eager(x))
+    assert a.lengths == b.lengths == a.kv_len.tolist() and status_ok()
+    for ca, cb in zip(a.caches, b.caches):
+        assert torch.equal(ca.k_pages.view(torch.uint8), cb.k_pages.view(torch.uint8)) and torch.equal(ca.k_scale, cb.k_scale)
+    with pytest.raises(ValueError):
+        a.prompt(n(100, 256).to(F16), [100, 0, 0])
+    with pytest.raises(ValueError):
+        a.prompt(n(4, 256).to(F16), [1, 1, 1])
+    with pytest.raises(ValueError):
+        a.step(n(2, 256).to(F16))

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace ob_block {
 
 // A cache page holds 64 tokens: keys (page, head, 64, dim), values (page, head, dim, 64), both e4m3, one fp32 scale for
@@ -111,6 +113,18 @@ cudaError_t launch_following(void (*kernel)(Params...), dim3 grid, int threads, 
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device (a bit of `ready` for each).
+template <typename K> cudaError_t allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 }  // namespace ob_block

@@ -15,6 +15,7 @@
 // Long caches with too few row tiles to fill the chip are split along the cached tokens; the parts are joined by a second kernel.
 // Every mbarrier wait is bounded. No TMA.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "block_common.h"
@@ -547,7 +548,8 @@ int many_splits(const ob::CacheAttendCall& c) {
 template <typename T, int D> cudaError_t launch_many(const ob::CacheAttendCall& c, void* workspace, cudaStream_t stream) {
   const int splits = many_splits(c);
   float* partial = static_cast<float*>(workspace);
-  cudaError_t e = cudaFuncSetAttribute(ob_attend_many_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_shared_memory(ob_attend_many_kernel<T, D>, Cfg<D>::kSmem, ready);
   if (e != cudaSuccess) return e;
   ob_attend_many_kernel<T, D><<<dim3((unsigned)(many_slots(c) * c.kv_heads), splits), kThreads, Cfg<D>::kSmem, stream>>>(c, partial, splits);
   e = cudaGetLastError();

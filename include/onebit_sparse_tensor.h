@@ -244,7 +244,7 @@ int onebit_cache_append(const void *k, int64_t k_token_stride, int64_t k_head_st
                         int64_t head_dim, int dtype, void *stream);
 
 /* out (tokens, heads, head_dim) = softmax(scale * q k^T) v over each sequence's cache; head h reads cache head
- * h / (heads / kv_heads). causal: a new token at position p sees the positions up to p (the new tokens are the last of
+ * h / group, group = heads / kv_heads, tokens * group^2 < 2^40. causal: a new token at position p sees the positions up to p (the new tokens are the last of
  * kv_len), else all kv_len. A row that sees nothing gets zeros. q, out: 16-byte aligned, strides multiples of 8.
  * max_new: the caller's bound of a sequence's new tokens (0: tokens); it only selects the kernel, results are right for any value.
  * workspace: device memory of onebit_cache_attend_workspace bytes (may be 0), 256-byte aligned, for this call until its work on

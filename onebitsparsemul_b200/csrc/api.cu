@@ -432,6 +432,8 @@ int onebit_cache_attend(const void* q, int64_t q_token_stride, int64_t q_head_st
   if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) return fail(ONEBIT_ERR_ARG, "pages must be 16-byte aligned");
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) || ((q_token_stride | q_head_stride | out_token_stride | out_head_stride) & 7))
     return fail(ONEBIT_ERR_ARG, "q and out must be 16-byte aligned with strides that are multiples of 8");
+  const int64_t group = heads / kv_heads;
+  if (tokens * group * group >= (1ll << 40)) return fail(ONEBIT_ERR_SHAPE, "%lld tokens of %lld query heads per cache head are too many", (long long)tokens, (long long)group);
   if (tokens == 0) return ONEBIT_OK;
   ob::CacheAttendCall c = attend_shape(pages, table_width, tokens, seqs, heads, kv_heads, head_dim, max_new);
   c.q = q, c.out = out, c.q_ts = q_token_stride, c.q_hs = q_head_stride, c.o_ts = out_token_stride, c.o_hs = out_head_stride;

@@ -71,7 +71,7 @@ struct alignas(16) Header {
 
 struct FewLayout {                                // the workspace, and what the host works out once
   int group;                                      // query heads of a cache head
-  uint64_t per_group;                             // ceil(2^40 / group): row / group = row * per_group >> 40 for rows below 2^28
+  uint64_t per_group;                             // ceil(2^40 / group): row / group = row * per_group >> 40 while row * group < 2^40
   Header* headers;
   float* partial;                                 // slots 2 c (segment that started before CTA c), 2 c + 1: rows x (D + 4): M, l at [D], [D + 1]
 };
@@ -133,7 +133,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
   for (int s = s_lo; s < s_hi; ++s) {
     const Seq q = seq_info(c, group, s, kRows);
     mine += q.w;
-    bad |= q.n == 0 && (__ldg(c.q_start + s) < 0 || __ldg(c.q_start + s + 1) > c.tokens);
+    bad |= (q.n == 0 && (__ldg(c.q_start + s) < 0 || __ldg(c.q_start + s + 1) > c.tokens)) || (q.n > 0 && q.kv > c.table_width * kPageTokens);
   }
   if (bad && blockIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
   int64_t upto = mine;

@@ -147,6 +147,7 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   const int n = q1 - q0, rows_all = n * group, row0 = tile * kCtaRows;
   if (tile < 0 || row0 >= rows_all) return;                     // tile < 0: q_start runs backwards
   const int kv = (int)min((int64_t)max(kv_raw, 0), c.table_width * kPageTokens);
+  if (kv < kv_raw && threadIdx.x == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
   auto limit_of = [&](int r) { return c.causal ? min(kv, kv_raw - n + r / group + 1) : kv; };
   const int hi = max(0, limit_of(min(rows_all, row0 + kCtaRows) - 1));
   const int steps_all = (hi + kTileTokens - 1) / kTileTokens;

@@ -2,6 +2,7 @@
 // the call into the C ABI of libonebitmul. The documented functions are those of onebitsparsemul_b200/block_ops.py, which
 // hand their arguments through: in a decode step these calls are a few microseconds of GPU work each, and checks and ctypes
 // conversions in Python took longer than that (a norm of one token: 21 us a call from Python through ctypes).
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -47,6 +48,13 @@ int type_code(const Tensor& t) {
   return ONEBIT_DENSE_BF16;
 }
 
+// An output has a place of its own for every value, and is an input as a whole or not at all.
+void check_output(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+  TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, name, " has several values in one place");
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_VALUE(!t || at::get_overlap_status(out, *t) != at::MemOverlapStatus::Partial, name, " overlaps an input without being it");
+}
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // t as (rows, hidden) with contiguous rows
@@ -78,6 +86,9 @@ py::object residual_norm(const Tensor& x, const Tensor& weight, const OptTensor&
     h = residual_out ? *residual_out : torch::empty(x.sizes(), residual->options());
     r2 = rows_of(*residual, hidden);
   }
+  if (out) check_output(*out, "out", {&x, residual, gate, residual_out});
+  if (residual_out) check_output(*residual_out, "residual_out", {&x, residual, gate});
+  TORCH_CHECK_VALUE(!out || !residual_out || out->numel() == 0 || out->data_ptr() != residual_out->data_ptr(), "out and residual_out must be different tensors");
   Tensor g2;
   int64_t gate_stride = 0;
   if (gate) {
@@ -119,6 +130,7 @@ void check_turned(const Tensor& out, const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && (out.stride(2) == 1 || out.size(2) == 1), name,
                     " must have the input's shape and type and contiguous heads");
   TORCH_CHECK_VALUE(out.data_ptr() != x.data_ptr() || out.strides() == x.strides(), name, " overlaps the input without being it");
+  check_output(out, name, {&x});
 }
 
 Tensor rotary_tokens(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, const std::string& layout, double magnitude, const OptTensor& out_) {
@@ -227,6 +239,7 @@ Tensor cache_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
   TORCH_CHECK_VALUE(!out || (out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->is_contiguous() && aligned(*out)),
                     "out must be contiguous (and 16-byte aligned) with q's shape and type");
+  TORCH_CHECK_VALUE(!out || at::get_overlap_status(*out, q) == at::MemOverlapStatus::No || at::get_overlap_status(*out, q) == at::MemOverlapStatus::TooHard, "out overlaps q");
   Tensor y = out ? *out : torch::empty(q.sizes(), q.options());
   if (tokens > 0) {
     const bool as_it_is = q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && aligned(q);

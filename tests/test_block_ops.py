@@ -61,6 +61,7 @@ def test_attend_refusals_on_the_host(lib):
     assert call(q=None) == 2 and call(kv_len=None) == 2
     assert call(dim=32) == 1 and call(heads=9) == 1 and call(seqs=70000) == 1 and call(width=1 << 25) == 1
     assert call(q=ODD) == 5 and call(q_ts=516) == 5 and call(k_pages=ODD) == 5 and call(dtype=3) == 5
+    assert call(tokens=1 << 20, heads=4096, kv_heads=4) == 1          # 2^20 tokens of 1024 heads: 2^40
     assert call(tokens=0) == 0
     need = lib.onebit_cache_attend_workspace(4, 4, 2, 8, 2, 64, 0)
     if need:

@@ -292,6 +292,43 @@ def test_bad_pages_and_ranges_are_left_out():
     assert status_ok()
 
 
+@pytest.mark.parametrize("new", [1, 80])
+def test_a_sequence_longer_than_its_table_is_reported(new):
+    cache, table = random_cache([128], 2, 64, 3)
+    batch = ob.CacheBatch(i32(0, new), i32(190), table, new)          # two pages for 190 tokens
+    q = gen(4)(new, 4, 64).to(F16)
+    want = plain.Cache(cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale)
+    out, spread, delta, least, _ = plain.attend(q, want, batch.q_start, batch.kv_len, table, 0.125, True)
+    got = ob.cache_attend(q, cache, batch)
+    assert ((got.cpu().double() - out).abs() <= plain.attend_tolerance(out, spread, delta, least, F16)).all()
+    assert not status_ok() and status_ok()
+    k = gen(5)(new, 2, 64).to(F16)
+    ob.cache_append(k, k, cache, batch)
+    assert not status_ok() and status_ok()
+
+
+def test_outputs_that_overlap_are_refused():
+    n = gen(9)
+    x, w, r = n(8, 64).to(F16), n(64).to(F16), n(8, 64).to(F16)
+    y = torch.empty_like(x)
+    flat = n(9 * 64).to(F16)
+    for kw in (dict(out=y, residual_out=y), dict(x=flat[:512].view(8, 64), out=flat[64:].view(8, 64)), dict(residual=flat[:512].view(8, 64), residual_out=flat[64:].view(8, 64))):
+        with pytest.raises(ValueError):
+            ob.residual_norm(**{**dict(x=x, weight=w, residual=r), **kw})
+    pos, freq = torch.arange(8, device=DEV), ob.rotary_frequencies(64)[0]
+    with pytest.raises(ValueError):
+        ob.rotary_tokens(x.view(8, 1, 64), pos, freq, out=n(1, 1, 64).to(F16).expand(8, 1, 64))
+    with pytest.raises(ValueError):
+        ob.rotary_tokens(flat[:512].view(8, 1, 64), pos, freq, out=flat[64:].view(8, 1, 64))
+    cache = ob.KVCache8.empty(1, 1, 64)
+    batch = ob.CacheBatch(i32(0, 8), i32(8), i32(0).view(1, 1))
+    q = x.view(8, 1, 64)
+    with pytest.raises(ValueError):
+        ob.cache_attend(q, cache, batch, out=q)
+    with pytest.raises(ValueError):
+        ob.cache_append(q, q, cache, batch, q=q, inv_freq=freq, q_out=n(1, 1, 64).to(F16).expand(8, 1, 64))
+
+
 def test_append_refusals():
     n = gen(13)
     cache = ob.KVCache8.empty(4, 2, 64)

@@ -55,7 +55,7 @@ __device__ __forceinline__ Seq seq_info(const ob::CacheAttendCall& c, int group,
   const int q1 = __ldg(c.q_start + s + 1);
   q.q0 = __ldg(c.q_start + s);
   q.kv = __ldg(c.kv_len + s);
-  q.n = q.q0 < 0 || q1 > c.tokens || q1 < q.q0 ? 0 : q1 - q.q0;
+  q.n = q.q0 < 0 || q1 > c.tokens || q1 < q.q0 || (int64_t)(q1 - q.q0) * group > c.few_rows ? 0 : q1 - q.q0;
   const int64_t room = c.table_width * kPageTokens;
   const int seen = (int)min((int64_t)max(q.kv, 0), room);
   q.pages = q.n > 0 ? max(1, (seen + kPageTokens - 1) / kPageTokens) : 0;
@@ -564,8 +564,20 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256) o
   }
 }
 
-// Which kernel: both are right for any batch.
-bool many_rows(const ob::CacheAttendCall& c) { return c.max_new * (c.heads / c.kv_heads) > 32; }
+// Which kernel has which sequences. This file's has those of up to 48 query rows per cache head, the tensor-memory kernel the
+// longer ones: 16 sequences of 8 / 12 / 16 / 24 tokens, contexts of 8192, 32 / 8 heads of 128, take 89 / 137 / 173 / 245 us here
+// and 161 / 158 / 159 / 164 us there.
+// A batch whose bound is above that may hold both kinds, a prompt among single tokens. Where the bound is far above the mean and
+// the sequences are enough to fill the GPU on their own, both kernels run, each for its sequences: n single tokens and a prompt
+// of 512 (contexts of 4096) take 138 -> 104 us for n = 14, 297 -> 185 us for 64; with contexts of 512 and n = 24, 31 -> 38 us.
+// Fewer hide behind the prompt's tiles: n = 6 takes 102 us in the prompt's kernel alone, 110 us in both.
+constexpr int kFewRows = 48;
+struct Plan { bool few, many; int few_rows; };
+Plan plan_of(const ob::CacheAttendCall& c) {
+  if (c.max_new * (c.heads / c.kv_heads) <= kFewRows) return {true, false, 0x7fffffff};
+  const bool both = 4 * c.tokens < c.seqs * c.max_new && 3 * c.seqs * c.kv_heads >= 2 * ob::sm_count();
+  return {both, true, both ? kFewRows : 0};
+}
 int few_tiles(const ob::CacheAttendCall& c) { return c.max_new * (c.heads / c.kv_heads) <= 8 ? 1 : 2; }
 // two CTAs per SM, but no more pieces than the block table could fill
 int few_grid(const ob::CacheAttendCall& c) {
@@ -596,14 +608,20 @@ template <typename T, int D, int NT> cudaError_t launch_few(const ob::CacheAtten
 
 namespace ob {
 
-int64_t cache_attend_workspace(const CacheAttendCall& c) {
-  if (many_rows(c)) return cache_attend_many_workspace(c);
+static int64_t few_workspace(const CacheAttendCall& c) {
   const int64_t grid = few_grid(c);
   return ((grid * (int64_t)sizeof(Header) + 255) & ~255ll) + 2 * grid * 8 * few_tiles(c) * (c.head_dim + 4) * 4;
 }
 
-cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream) {
-  if (many_rows(c)) return launch_cache_attend_many(c, workspace, stream);
+int64_t cache_attend_workspace(const CacheAttendCall& c) {
+  const Plan p = plan_of(c);
+  return (p.few ? (few_workspace(c) + 255) & ~255ll : 0) + (p.many ? cache_attend_many_workspace(c) : 0);
+}
+
+cudaError_t launch_cache_attend(const CacheAttendCall& call, void* workspace, cudaStream_t stream) {
+  const Plan p = plan_of(call);
+  CacheAttendCall c = call;
+  c.few_rows = p.few_rows;
   auto by_tiles = [&](auto t, auto d) {
     return few_tiles(c) == 1 ? launch_few<decltype(t), decltype(d)::value, 1>(c, workspace, stream)
                              : launch_few<decltype(t), decltype(d)::value, 2>(c, workspace, stream);
@@ -611,13 +629,20 @@ cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaS
   auto by_dim = [&](auto t) {
     return c.head_dim == 64 ? by_tiles(t, std::integral_constant<int, 64>{}) : by_tiles(t, std::integral_constant<int, 128>{});
   };
-  return c.bf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
+  if (p.few) {
+    cudaError_t e = c.bf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
+    if (e != cudaSuccess || !p.many) return e;
+    workspace = static_cast<uint8_t*>(workspace) + ((few_workspace(c) + 255) & ~255ll);
+  }
+  return launch_cache_attend_many(c, workspace, stream);
 }
 
 cudaError_t read_attend_status(int* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_attend_status, sizeof(int));
-  if (e != cudaSuccess) return e;
-  if (*out == 0) return read_attend_many_status(out);
+  int few = 0;
+  cudaError_t e = read_attend_many_status(out);                 // a batch may have been both kernels'
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&few, g_attend_status, sizeof(int));
+  if (e != cudaSuccess || few == 0) return e;
+  *out = few;
   const int zero = 0;
   return cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
 }

@@ -145,6 +145,7 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
     return;
   }
   const int n = q1 - q0, rows_all = n * group, row0 = tile * kCtaRows;
+  if (rows_all <= c.few_rows) return;                           // cache_attend.cu's
   if (tile < 0 || row0 >= rows_all) return;                     // tile < 0: q_start runs backwards
   const int kv = (int)min((int64_t)max(kv_raw, 0), c.table_width * kPageTokens);
   if (kv < kv_raw && threadIdx.x == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
@@ -519,7 +520,7 @@ template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_jo
   for (int s0 = 0; s0 <= c.seqs; s0 += 32) first += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && __ldg(c.q_start + min((int64_t)s0 + lane, c.seqs)) <= t));
   if (first < 1 || first > c.seqs) return;                      // padding: not written
   const int q0 = __ldg(c.q_start + first - 1), q1 = __ldg(c.q_start + first);
-  if (q0 < 0 || q1 > c.tokens) return;
+  if (q0 < 0 || q1 > c.tokens || (q1 - q0) * (c.heads / c.kv_heads) <= c.few_rows) return;
   const float* p = partial + row * (D + 4);
   const int64_t step = rows * (D + 4);
   float M = -INFINITY;

@@ -99,6 +99,7 @@ struct CacheAttendCall {
   int64_t max_new;             // the caller's bound of a sequence's new tokens: it picks the kernel, no result depends on it
   float scale;
   bool causal, bf16;
+  int few_rows;                // sequences with at most this many query rows per cache head are one kernel's, the others the other's
 };
 int64_t cache_attend_workspace(const CacheAttendCall& c);
 cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream);

@@ -410,6 +410,30 @@ def test_attend_hint_and_padding_do_not_change_what_is_right(hint):
     check_attend([1, 30, 2, 90], [100, 230, 2, 90], 8, 2, 128, F16, max_new=hint, seed=3, pad=(3, 5))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,causal", [(16, 8, 128, F16, True), (32, 32, 64, BF16, True), (40, 10, 64, F16, False), (24, 8, 128, BF16, False)])
+def test_attend_prompts_among_single_tokens(heads, kv_heads, dim, dtype, causal):
+    """Batches that both kernels share, each its sequences: lengths on either side of the rule, empty ones, padded rows."""
+    new = [1, 0, 150, 1, 12, 13, 1, 24, 25, 1, 1, 16, 17, 1, 48, 49, 2, 1, 1, 1]
+    kv = [700, 5, 1000, 64, 12, 80, 1, 100, 25, 300, 129, 10, 17, 0, 48, 200, 65, 900, 33, 63]
+    q, cache, batch, got = check_attend(new, kv, heads, kv_heads, dim, dtype, causal=causal, max_new=150, seed=dim, pad=(2, 3))
+    written = slice(2, 2 + sum(new))
+    for _ in range(5):
+        assert torch.equal(ob.cache_attend(q, cache, batch, causal=causal)[written], got[written])
+    check_attend([1] * 40 + [200], list(range(1, 1601, 40)) + [333], heads, kv_heads, dim, dtype, causal=causal, max_new=200, seed=7)
+    want = plain.Cache(cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale)
+    out, spread, delta, least, _ = plain.attend(q, want, batch.q_start, batch.kv_len, batch.block_table, dim ** -0.5, causal)
+    tol = plain.attend_tolerance(out, spread, delta, least, dtype)
+    batch.q_start[3] = -1                                       # bad sequences in the middle: two have no range, the others stay right
+    again = torch.full_like(got, 9.0)
+    ob.cache_attend(q, cache, batch, causal=causal, out=again)
+    assert not status_ok() and status_ok()
+    ends = [2 + sum(new[:i]) for i in range(len(new) + 1)]
+    assert (again[ends[2]:ends[4]] == 9.0).all()
+    # right, not the same bits: the sums are cut into pieces where the whole batch says, each of them within the bound
+    for keep in (slice(ends[0], ends[2]), slice(ends[4], ends[-1])):
+        assert ((again.cpu().double() - out).abs() <= tol)[keep].all()
+
+
 @pytest.mark.parametrize("scale,size", [(0.0, 1.0), (-0.1, 1.0), (3.0, 2.0), (1e-3, 300.0), (1e-4, 6e4)])
 def test_attend_scales_and_large_queries(scale, size):
     for new, kv in (([1, 2], [300, 90]), ([140], [200])):

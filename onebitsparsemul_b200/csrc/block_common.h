@@ -104,25 +104,33 @@ __device__ __forceinline__ void follow_previous_kernel() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+struct ClusterOf { int ctas; };
 template <typename... Params, typename... Args>
-cudaError_t launch_following(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+cudaError_t launch_following(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, ClusterOf cluster, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
+  cudaLaunchAttribute attrs[2]{};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = (unsigned)cluster.ctas, attrs[1].val.clusterDim.y = 1, attrs[1].val.clusterDim.z = 1;
+  cfg.attrs = attrs, cfg.numAttrs = cluster.ctas > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+template <typename... Params, typename... Args>
+cudaError_t launch_following(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  return launch_following(kernel, grid, threads, smem, stream, ClusterOf{1}, args...);
+}
 
-// Raises a kernel's dynamic shared memory limit, once per device (a bit of `ready` for each).
-template <typename K> cudaError_t allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t>& ready) {
+// Raises a kernel's dynamic shared memory limit, once per device (a bit of `ready` for each); and allows clusters of 16.
+template <typename K> cudaError_t allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t>& ready, bool wide_clusters = false) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (ready.load(std::memory_order_acquire) & bit) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
   return e;
 }

@@ -396,6 +396,16 @@ def test_attend_few_rows(new, kv, heads, kv_heads, dim, dtype):
     check_attend(new, kv, heads, kv_heads, dim, dtype, max_new=max(1, max(new)), seed=len(kv) + kv[0])
 
 
+@pytest.mark.parametrize("new,kv,hint", [  # clusters of every size, more and fewer CTAs than pages, more row tiles than the bound says
+    ([1], [2500], 1), ([1], [300], 1), ([3], [700], 1), ([20], [2100], 1), ([1, 1], [4000, 3], 1), ([20, 2], [2100, 130], 2), ([9, 1, 0, 1], [1025, 0, 5, 640], 9),
+    ([1] * 5, [0, 1, 600, 1025, 130], 1), ([1] * 12, list(range(60, 1260, 100)), 1), ([17] * 3, [400, 17, 1100], 3), ([1] * 40, [4200] + list(range(1, 391, 10)), 1)])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(8, 8, 128, BF16), (8, 2, 64, F16), (5, 1, 128, F16), (48, 16, 64, BF16)])
+def test_attend_few_rows_by_clusters(new, kv, hint, heads, kv_heads, dim, dtype):
+    q, cache, batch, got = check_attend(new, kv, heads, kv_heads, dim, dtype, max_new=hint, seed=kv[0], pad=(1, 2))
+    for _ in range(3):
+        assert torch.equal(ob.cache_attend(q, cache, batch)[1:1 + sum(new)], got[1:1 + sum(new)])
+
+
 MANY = [([200], [200]), ([130], [1000]), ([64, 1, 65], [64, 600, 65]), ([300, 0, 7, 129], [300, 5, 900, 129]), ([100], [60]), ([128], [128]), ([256], [256]), ([257], [640])]
 
 

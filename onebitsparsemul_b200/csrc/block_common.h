@@ -83,6 +83,7 @@ __device__ __forceinline__ float2 cos_sin(uint64_t per_position, int64_t positio
 
 // ---- e4m3 -----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) { return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float from_e4m3(uint8_t c) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
   return __half2float(__half(h));

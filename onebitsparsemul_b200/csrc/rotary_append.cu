@@ -62,7 +62,7 @@ struct AppendArgs {
   int page_slots;                      // CTAs of the append half of the grid: page slots x kv_heads
 };
 
-constexpr int kAppendTokens = 2, kFewTokens = 4;   // query tokens per CTA of an append: with prompts, with steps
+constexpr int kAppendTokens = 4, kFewTokens = 4;   // query tokens per CTA of an append: with prompts, with steps
 constexpr int kRotThreads = 256;
 constexpr int kMaxHalf = 256;
 constexpr int kBatch = 4;              // pieces that a thread has under way
@@ -214,10 +214,22 @@ template <int THREADS> __device__ __forceinline__ float cta_max(float v, float (
   return v;
 }
 
-// 2 D threads: 16 groups of 4 tokens (a word of the transposed values) x D / 8 groups of 8 values. Bound by the queries' bytes on
-// prompts and by its chain of dependent loads (batch, page, tokens) on single tokens; at 64 registers four CTAs share an SM.
+// the larger magnitudes of two pairs of values; a NaN stays
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b, __half) {
+  const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), __habs2(*reinterpret_cast<const __half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// 2 D threads: 16 groups of 4 tokens (a word of the transposed values) x D / 8 groups of 8 values. The grid is in two halves:
+// 8 prompts of up to 2048 tokens (8 heads of 128, 32 query heads) take 43.7 us, of which the queries alone are 30 (the rate of the
+// rotation by itself) and the pages' instructions the rest; the pages among the queries instead of before them: 44.9 us. At 80
+// registers three CTAs of 256 threads share an SM and a thread has all kBatch pieces of 4 tokens' queries under way; four CTAs at
+// 64 registers spill (49.2 us, with two tokens 46.7), two at 128 are too few (50.3 us).
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(const AppendArgs a, const RotaryArgs q) {
+__global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(const AppendArgs a, const RotaryArgs q) {
   follow_previous_kernel();
   constexpr int kThreads = 2 * D;
   __shared__ __align__(16) float2 cs[kPageTokens][D / 2];
@@ -276,6 +288,8 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
   const int quad = (tid & 7) + 8 * ((tid >> 5) / (kVecs / 4)); // a warp: 8 x 4 of the groups
   const int vec = ((tid >> 3) & 3) + 4 * ((tid >> 5) % (kVecs / 4));
   const int d0 = vec * 8;
+  // where pair i of a token lies in its row of the table: the eight tokens that a warp reads at a time are in different banks
+  auto at = [](int place, int i) { return i ^ ((place >> 2 & 7) << 1); };
 
   for (int64_t block = max(before, 0) / kPageTokens + mine; block * kPageTokens < kv; block += slots) {
     const int base = (int)block * kPageTokens;
@@ -320,22 +334,33 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
     }
     if (tid < kPageTokens) nan_token[tid] = 0;
     for (int i = tid % (D / 2); i < r.half; i += D / 2)       // D / 2 pairs of 4 tokens at a time
-      for (int tt = lo + tid / (D / 2); tt < hi; tt += 4) cs[tt][i] = cos_sin(turns_per_position(r.freq[i]), (int64_t)base + tt, r.magnitude);
+      for (int tt = lo + tid / (D / 2); tt < hi; tt += 4) cs[tt][at(tt, i)] = cos_sin(turns_per_position(r.freq[i]), (int64_t)base + tt, r.magnitude);
     __syncthreads();
 
-    float v_max = 0.f;
+    uint32_t v_top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&vr[i]);
-      bool nan = false;
+      const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack2(w[e], T{});
-        v_max = finite_max(finite_max(v_max, f.x), f.y);
-        if (isnan(f.x)) { w[e] &= 0xFFFF0000u; nan = true; }  // stored as 0
-        if (isnan(f.y)) { w[e] &= 0x0000FFFFu; nan = true; }
+      for (int e = 0; e < 4; ++e) v_top = abs_max2(v_top, w[e], T{});
+    }
+    float2 top = unpack2(v_top, T{});
+    float v_max = fmaxf(top.x, top.y);
+    if (!(top.x <= 3.402823466e38f && top.y <= 3.402823466e38f)) {               // an infinity or a NaN among the 32
+      v_max = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&vr[i]);
+        bool nan = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2(w[e], T{});
+          v_max = finite_max(finite_max(v_max, f.x), f.y);
+          if (isnan(f.x)) { w[e] &= 0xFFFF0000u; nan = true; }  // stored as 0
+          if (isnan(f.y)) { w[e] &= 0x0000FFFFu; nan = true; }
+        }
+        if (nan) nan_token[quad * 4 + i] = 1;
       }
-      if (nan) nan_token[quad * 4 + i] = 1;
     }
     // keys, turned
     float kf[4][8], k_max = 0.f;
@@ -352,10 +377,9 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
         const T* k = static_cast<const T*>(a.k) + (row0 + place) * a.k_ts + (int64_t)head * a.k_hs;
         if constexpr (W == 8) {
           if (r.interleaved) {
-            const float4* c4 = reinterpret_cast<const float4*>(&cs[place][d0 / 2]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float4 c = c4[e / 2];
+              const float4 c = *reinterpret_cast<const float4*>(&cs[place][at(place, d0 / 2 + (e & 2))]);
               const float cc = e & 1 ? c.z : c.x, ss = e & 1 ? c.w : c.y, x = kf[i][2 * e], y = kf[i][2 * e + 1];
               kf[i][2 * e] = x * cc - y * ss;
               kf[i][2 * e + 1] = y * cc + x * ss;
@@ -366,9 +390,10 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
             float other[8];
             load8(k + (front ? d0 + r.half : p0), other);     // a neighbour's piece: from the first-level cache
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 c = cs[place][p0 + e];
+            for (int e = 0; e < 8; e += 2) {
+              const float4 c = *reinterpret_cast<const float4*>(&cs[place][at(place, p0 + e)]);
               kf[i][e] = front ? kf[i][e] * c.x - other[e] * c.y : kf[i][e] * c.x + other[e] * c.y;
+              kf[i][e + 1] = front ? kf[i][e + 1] * c.z - other[e + 1] * c.w : kf[i][e + 1] * c.z + other[e + 1] * c.w;
             }
           }
         } else {
@@ -378,7 +403,7 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
             if (d < 2 * r.half) {
               const int p = r.interleaved ? d / 2 : (d < r.half ? d : d - r.half);
               const bool front = r.interleaved ? (d & 1) == 0 : d < r.half;
-              const float2 c = cs[place][p];
+              const float2 c = cs[place][at(place, p)];
               const float other = to_f32(k[r.interleaved ? d ^ 1 : (front ? d + r.half : d - r.half)]);
               kf[i][e] = front ? kf[i][e] * c.x - other * c.y : kf[i][e] * c.x + other * c.y;
             }
@@ -386,7 +411,14 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) k_max = finite_max(k_max, kf[i][e]);
+      for (int e = 0; e < 8; ++e) k_max = fmaxf(k_max, fabsf(kf[i][e]));        // passes a NaN over
+    }
+    if (k_max > 3.402823466e38f) {                            // an infinity: the largest value next to it
+      k_max = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k_max = finite_max(k_max, kf[i][e]);
     }
     v_max = cta_max<kThreads>(v_max, red[0]);
     k_max = cta_max<kThreads>(k_max, red[1]);                 // both CTA barriers: every thread has read the old scales
@@ -411,7 +443,7 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
       uint32_t c[2] = {0, 0};
       if (is_new) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e / 4] |= (uint32_t)to_e4m3(kf[i][e] * k_inv) << (8 * (e & 3));
+        for (int e = 0; e < 8; e += 2) c[e / 4] |= to_e4m3x2(kf[i][e] * k_inv, kf[i][e + 1] * k_inv) << (8 * (e & 3));
         if (d0 == 0 && nan_token[place]) c[0] = (c[0] & ~0xFFu) | 0x7Fu;
       } else if (place < lo) {
         const uint2 old = *at;
@@ -424,8 +456,19 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
     // values: 4 tokens of each of 8 rows
     const bool any_new = quad * 4 < hi && quad * 4 + 4 > lo;
     if (any_new || fresh || (quad * 4 < lo && v_ratio != 1.f)) {
-      const bool whole = fresh || (quad * 4 >= lo && quad * 4 + 4 <= hi);
+      const bool all_new = quad * 4 >= lo && quad * 4 + 4 <= hi, whole = fresh || all_new;
       uint8_t* vp = a.v_pages + ph * (kPageTokens * D) + quad * 4;
+      if (all_new) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float2 f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = unpack2(reinterpret_cast<const uint32_t*>(&vr[i])[e / 2], T{});
+          uint32_t* at = reinterpret_cast<uint32_t*>(vp + (d0 + e) * kPageTokens);
+          at[0] = to_e4m3x2(f[0].x * v_inv, f[1].x * v_inv) | to_e4m3x2(f[2].x * v_inv, f[3].x * v_inv) << 16;
+          at[kPageTokens / 4] = to_e4m3x2(f[0].y * v_inv, f[1].y * v_inv) | to_e4m3x2(f[2].y * v_inv, f[3].y * v_inv) << 16;
+        }
+      } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         uint32_t* at = reinterpret_cast<uint32_t*>(vp + (d0 + e) * kPageTokens);
@@ -445,6 +488,7 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D)) ob_cache_append_kernel(
           w |= (uint32_t)code << (8 * i);
         }
         *at = w;
+      }
       }
     }
     __syncthreads();                                          // the next page's tables go over this one's

@@ -60,8 +60,10 @@ template <> struct Raw<float, 8> {
 };
 
 // V chunks of W values per thread; chunk j of thread t starts at value (j * threads_of_row + t) * W. W = 8: 16-byte accesses
-// (hidden % 8 == 0 and every row aligned); W = 1: any width and alignment. Bound by memory on many rows: what a row is read into
-// stays packed until its sum is there, so that few registers a thread let enough rows be under way on an SM.
+// (hidden % 8 == 0 and every row aligned); W = 1: any width and alignment, bound by its 2-byte accesses (1111 x 2047: 2.9 TB/s).
+// Bound by memory on many rows: what a row is read into stays packed until its sum is there, so that few registers a thread let
+// enough rows be under way on an SM (8192 x 4096 with post norm and gate: 268 MB in 47.7 us, 5.6 TB/s, 86 % of the copy rate). One
+// row of 4096 takes 1.8 us: the launch and two dependent loads.
 template <typename T, typename R, int V, int W, bool WARP_ROW>
 __global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a) {
   __shared__ float scratch[2][32];
@@ -151,6 +153,66 @@ __global__ void __launch_bounds__(1024) ob_residual_norm_kernel(const NormArgs a
   }
 }
 
+// Rows above 4096 values that are not aligned: h waits in shared memory (fp32, up to 128 KB), since in registers it would be up to
+// 32 values a thread next to as many of x and the residual. 1111 rows of 8191 fp16 values with a residual: 22.7 us, in registers
+// (spilled) 113 us.
+constexpr int kLongThreads = 512;
+template <typename T, typename R> __global__ void __launch_bounds__(kLongThreads) ob_residual_norm_long_kernel(const NormArgs a) {
+  extern __shared__ float hs[];
+  __shared__ float scratch[2][32];
+  follow_previous_kernel();
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const R* res = a.residual ? static_cast<const R*>(a.residual) + row * a.r_stride : nullptr;
+  const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.g_stride : nullptr;
+  const T* post = static_cast<const T*>(a.post_weight);
+  const T* weight = static_cast<const T*>(a.weight);
+  T* y = static_cast<T*>(a.y) + row * a.y_stride;
+  R* hout = res ? static_cast<R*>(a.h) + row * a.h_stride : nullptr;
+  const float inv_n = 1.f / (float)a.hidden;
+  constexpr int kTogether = 8;                                 // loads under way
+  auto each = [&](auto load, auto use) {
+    for (int c0 = threadIdx.x; c0 < a.hidden; c0 += kTogether * kLongThreads) {
+      decltype(load(0)) v[kTogether];
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j)
+        if (c0 + j * kLongThreads < a.hidden) v[j] = load(c0 + j * kLongThreads);
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j)
+        if (c0 + j * kLongThreads < a.hidden) use(c0 + j * kLongThreads, v[j]);
+    }
+  };
+  float f = 1.f;
+  if (post) {
+    float s = 0.f;
+    each([&](int c) { return x[c]; }, [&](int, T v) { s += to_f32(v) * to_f32(v); });
+    f = rsqrtf(row_sum<false>(s, scratch[0]) * inv_n + a.eps);
+  }
+  struct In { T x, p, g; R r; };
+  float s = 0.f;
+  each([&](int c) {
+         In v{};
+         v.x = x[c];
+         if (res) v.r = res[c];
+         if (post) v.p = post[c];
+         if (gate) v.g = gate[c];
+         return v;
+       },
+       [&](int c, const In& v) {
+         float h = to_f32(v.x);
+         if (res) {
+           if (post) h *= f * to_f32(v.p);
+           if (gate) h *= to_f32(v.g);
+           h = to_f32(v.r) + a.residual_scale * h;
+           hout[c] = from_f32<R>(h);
+         }
+         hs[c] = h;
+         s += h * h;
+       });
+  f = rsqrtf(row_sum<false>(s, scratch[1]) * inv_n + a.eps);
+  each([&](int c) { return weight[c]; }, [&](int c, T w) { y[c] = from_f32<T>(to_f32(w) * (hs[c] * f)); });
+}
+
 template <typename T, typename R, int V, int W>
 cudaError_t launch_rows(const NormArgs& a, int threads, cudaStream_t stream) {
   constexpr int kRows = 4;                                    // rows (warps) per CTA where a warp has a row
@@ -164,11 +226,20 @@ template <typename T, typename R> cudaError_t launch_types(const NormArgs& a, bo
   const int chunks = wide ? a.hidden / 8 : a.hidden;
   auto threads_for = [&](int per) { return max(32, min(1024, ((chunks + per - 1) / per + 31) / 32 * 32)); };
   if (wide) {
-    if (chunks <= 1024) return launch_rows<T, R, 2, 8>(a, threads_for(2), stream);
+    // Values per thread: the fewest where a row's latency is all there is (64 x 4096 with a residual: 2.0 us with 8, 2.4 with 16,
+    // 2.8 with 32), more where the rows fill the GPU, for the sums' barriers (8192 x 4096, post norm and gate: 51.9 / 47.7 / 48.1 us;
+    // 1111 x 8192: 10.2 / 9.4 / 8.2 us).
+    if (a.rows <= 256 && chunks <= 1024) return launch_rows<T, R, 1, 8>(a, threads_for(1), stream);
+    if (chunks <= 512) return launch_rows<T, R, 2, 8>(a, threads_for(2), stream);
     return launch_rows<T, R, 4, 8>(a, threads_for(4), stream);
   }
+  // 1111 x 2047 bf16, fp32 residual, gate: 11.2 us with 4 values a thread, 12.6 with 8; 1111 x 4095 with a residual: 14.6 and 14.2
+  if (chunks <= 2048) return launch_rows<T, R, 4, 1>(a, threads_for(4), stream);
   if (chunks <= 4096) return launch_rows<T, R, 8, 1>(a, threads_for(8), stream);
-  return launch_rows<T, R, 32, 1>(a, threads_for(32), stream);
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = allow_shared_memory(ob_residual_norm_long_kernel<T, R>, 32768 * 4, ready);
+  if (e != cudaSuccess) return e;
+  return launch_following(ob_residual_norm_long_kernel<T, R>, dim3((unsigned)a.rows), kLongThreads, a.hidden * sizeof(float), stream, a);
 }
 
 }  // namespace

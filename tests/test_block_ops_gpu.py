@@ -62,6 +62,22 @@ def test_residual_norm(rows, hidden, dtype, wide, form):
     check_norm(y, h, x, weight, residual, gate, scale, post, 1e-5)
 
 
+@pytest.mark.parametrize("rows,hidden", [(300, 64), (259, 1024), (300, 4096), (257, 4104), (300, 2048), (270, 3001), (260, 4097), (600, 40)])
+def test_residual_norm_of_many_rows(rows, hidden):
+    for form in ("norm", "residual", "post", "full"):
+        test_residual_norm(rows, hidden, BF16, False, form)
+
+
+def test_residual_norm_of_long_unaligned_rows_in_place():
+    n = gen(4)
+    x, r, w, g = n(3, 9007).to(F16), n(3, 9007), (1 + 0.2 * n(9007)).to(F16), n(3, 9007).to(F16)
+    y, h = ob.residual_norm(x, w, residual=r, gate=g, post_weight=w, residual_scale=0.7)
+    x2, r2 = x.clone(), r.clone()
+    ob.residual_norm(x2, w, residual=r2, gate=g, post_weight=w, residual_scale=0.7, out=x2, residual_out=r2)
+    assert torch.equal(y, x2) and torch.equal(h, r2)
+    check_norm(y, h, x, w, r, g, 0.7, w, 1e-6)
+
+
 def test_residual_norm_shapes_strides_and_in_place():
     n = gen(1)
     rows = n(6, 6, 2 * 96 + 8).to(F16)
@@ -104,7 +120,8 @@ def test_residual_norm_refusals():
 
 def check_rotary(y, x, positions, freq, layout, magnitude=1.0):
     want, reach = plain.rotate(x.cpu(), positions.cpu(), freq.cpu(), layout, magnitude)
-    # cos and sin: phase in turns to 2^-32, its fp32 form to 2^-25 half turns, sincospi to 2 ulp, products and sum 3 roundings
+    # cos and sin: phase in turns to 2^-32, its fp32 form to 2^-25 half turns, cosf and sinf of the
+    # special function unit to 2^-21.2, products and sum 3 roundings
     tol = want.abs() * plain.HALF_STEP[x.dtype] * 1.01 + reach * 2.0 ** -20 + (2.0 ** -25 if x.dtype == F16 else 0)
     err = (y.double().cpu() - want).abs()
     assert (err <= tol).all(), float((err / tol.clamp(min=1e-30)).max())

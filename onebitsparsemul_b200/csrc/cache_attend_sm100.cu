@@ -512,6 +512,7 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
 
 // Joins the splits of a row: one warp per (token, head).
 template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_join_kernel(const ob::CacheAttendCall c, const float* partial, int splits) {
+  follow_previous_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = c.tokens * c.heads;
   if (row >= rows) return;
@@ -540,11 +541,23 @@ template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_jo
 
 int64_t many_slots(const ob::CacheAttendCall& c) { return c.tokens * (c.heads / c.kv_heads) / kCtaRows + c.seqs; }
 
+// Parts that the cache is cut into, for row tiles too few to fill the GPU: the number with the least estimated time, from what
+// was measured for heads of 128 values: 2.3 us a step of 128 tokens (64 values: 1.95), 11 us a CTA besides, and for the join 4 us
+// and the partial results at 1.7 TB/s. 32 / 8 heads, in 1 / 2 / 4 / 8 parts: 512 tokens over 4096 85 / 60 / 77 / 109 us (2 taken),
+// 128 over 4096 85 / 55 / 40 / 34 (8), 2048 over 2048 58 / 118 / 181 / 299 (1), 3 x 512 over 16384 598 / 503 / 551 / 619 (2; in 3
+// 472).
 int many_splits(const ob::CacheAttendCall& c) {
-  const int64_t ctas = many_slots(c) * c.kv_heads, sms = ob::sm_count();
-  if (ctas >= 2 * sms) return 1;
-  const int64_t most = std::max<int64_t>(1, (c.table_width + 15) / 16);          // at least 8 steps of 128 tokens each
-  return (int)std::min<int64_t>({(2 * sms + ctas - 1) / ctas, most, 64});
+  const int64_t group = c.heads / c.kv_heads, sms = ob::sm_count(), steps = (c.table_width + 1) / 2;
+  const int64_t ctas = ((c.tokens * group + kCtaRows - 1) / kCtaRows + (c.seqs - 1) / 2) * c.kv_heads;
+  const double step = c.head_dim == 128 ? 2.3 : 1.95, bytes = (double)c.tokens * c.heads * (c.head_dim + 4) * 4;
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= 64 && n <= steps; ++n) {
+    const double waves = ctas * n <= sms ? 1. : (double)(ctas * n) / sms + .5;
+    const double us = waves * ((steps + n - 1) / n * step + 11) + (n > 1 ? 4 + n * bytes / 1.7e6 : 0.);
+    if (n == 1 || us < least) best = n, least = us;
+  }
+  return best;
 }
 
 template <typename T, int D> cudaError_t launch_many(const ob::CacheAttendCall& c, void* workspace, cudaStream_t stream) {
@@ -556,8 +569,7 @@ template <typename T, int D> cudaError_t launch_many(const ob::CacheAttendCall& 
   ob_attend_many_kernel<T, D><<<dim3((unsigned)(many_slots(c) * c.kv_heads), splits), kThreads, Cfg<D>::kSmem, stream>>>(c, partial, splits);
   e = cudaGetLastError();
   if (e != cudaSuccess || splits == 1) return e;
-  ob_attend_join_kernel<T, D><<<(unsigned)((c.tokens * c.heads + 7) / 8), 256, 0, stream>>>(c, partial, splits);
-  return cudaGetLastError();
+  return launch_following(ob_attend_join_kernel<T, D>, dim3((unsigned)((c.tokens * c.heads + 7) / 8)), 256, 0, stream, c, partial, splits);
 }
 
 }  // namespace

@@ -145,7 +145,8 @@ class CacheBatch:
         block_table  (sequences, width) page of each 64 tokens; entries behind a sequence's length are never read
 
     max_new: an upper bound of the sequences' new tokens, if the caller knows one (a decode step: 1). It picks the
-    kernel, no result depends on it. Rows outside q_start's range are padding: not read, and their outputs not written. The
+    kernel, as the table's width does (the narrower, the better short batches are dealt out); results are right whatever it
+    says, though sums may be taken in another order. Rows outside q_start's range are padding: not read, and their outputs not written. The
     values stay on the device and may be rewritten between steps (a captured step reads them anew). A page number or a range
     that lies outside its tensor is left out, and ``onebit_check_device_status`` reports it."""
 

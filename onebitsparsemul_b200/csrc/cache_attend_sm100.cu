@@ -13,6 +13,9 @@
 //     multiplied, when it would otherwise let a weight pass 2^8: the sums are fp32, so a lower reference costs nothing.
 // Scales as in cache_attend.cu: the key scale multiplies the score, the value scale goes into the exponent.
 // Long caches with too few row tiles to fill the chip are split along the cached tokens; the parts are joined by a second kernel.
+// Measured: a prompt of 8192, 32 / 8 heads of 128, 592 us (930 TFLOP/s of the causal half, 56 % of the cuBLAS rate). No unit is
+// saturated: the softmax's instructions and the widening share the issue slots and wait for each other (leaving out either, or
+// the products, changes the time by 2 to 8 %).
 // Every mbarrier wait is bounded. No TMA.
 #include <algorithm>
 #include <atomic>

@@ -96,7 +96,7 @@ struct CacheAttendCall {
   int64_t pages;
   const int *q_start, *kv_len, *table;
   int64_t table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim;
-  int64_t max_new;             // the caller's bound of a sequence's new tokens: it picks the kernel, no result depends on it
+  int64_t max_new;             // the caller's bound of a sequence's new tokens: it picks the kernel, results are right whatever it is
   float scale;
   bool causal, bf16;
   int few_rows;                // sequences with at most this many query rows per cache head are one kernel's, the others the other's

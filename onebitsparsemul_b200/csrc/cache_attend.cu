@@ -46,6 +46,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ---- the line of pages ------------------------------------------------------------------------------------------------
 
 struct Seq {
+  bool bad;                                       // its range is not inside the call's rows, or its tokens not inside the table
   int q0, n, kv, pages, tiles;                    // kv: cached tokens; pages: 0 if the sequence has no new token, else at least 1
   int64_t w;                                      // pages of all its segments
 };
@@ -60,8 +61,10 @@ __device__ __forceinline__ Seq seq_info(const ob::CacheAttendCall& c, int group,
   const int q1 = __ldg(c.q_start + s + 1);
   q.q0 = __ldg(c.q_start + s);
   q.kv = __ldg(c.kv_len + s);
-  q.n = q.q0 < 0 || q1 > c.tokens || q1 < q.q0 || (int64_t)(q1 - q.q0) * group > c.few_rows ? 0 : q1 - q.q0;
+  q.bad = q.q0 < 0 || q1 > c.tokens || q1 < q.q0;
+  q.n = q.bad || (int64_t)(q1 - q.q0) * group > c.few_rows ? 0 : q1 - q.q0;
   const int64_t room = c.table_width * kPageTokens;
+  q.bad |= q.n > 0 && q.kv > room;
   const int seen = (int)min((int64_t)max(q.kv, 0), room);
   q.pages = q.n > 0 ? max(1, (seen + kPageTokens - 1) / kPageTokens) : 0;
   q.tiles = (q.n * group + rows_per_tile - 1) / rows_per_tile;
@@ -156,9 +159,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     const int p = page0 + stride * (warp + kWarps * lane);      // the first page numbers do not wait for the lengths
     if (p < c.table_width) first_id = __ldg(c.table + (int64_t)seq * c.table_stride + p);
     q = seq_info(c, group, seq, kRows);
-    if (page0 == 0 && tile == 0 && head == 0 && threadIdx.x == 0 &&
-        ((q.n == 0 && (q.q0 < 0 || __ldg(c.q_start + seq + 1) > c.tokens)) || (q.n > 0 && q.kv > c.table_width * kPageTokens)))
-      atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+    if (q.bad && page0 == 0 && tile == 0 && head == 0 && threadIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
     if (tile >= q.tiles) return;                                // the whole cluster
     b = (q.tiles - tile + ws.tiles - 1) / ws.tiles;             // more than one round where the caller's bound was wrong
     take = q.pages > page0 ? (q.pages - page0 + stride - 1) / stride : 0;
@@ -176,7 +177,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
   for (int s = s_lo; s < s_hi; ++s) {
     const Seq q = seq_info(c, group, s, kRows);
     mine += q.w;
-    bad |= (q.n == 0 && (__ldg(c.q_start + s) < 0 || __ldg(c.q_start + s + 1) > c.tokens)) || (q.n > 0 && q.kv > c.table_width * kPageTokens);
+    bad |= q.bad;
   }
   if (bad && blockIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
   int64_t upto = mine;

@@ -324,6 +324,22 @@ def test_a_sequence_longer_than_its_table_is_reported(new):
     assert not status_ok() and status_ok()
 
 
+@pytest.mark.parametrize("width,hint", [(8, 1), (200, 1), (8, 200)])
+def test_ranges_that_run_backwards_are_reported(width, hint):
+    cache, table = random_cache([300] * 40, 4, 64, 3)
+    wide = torch.zeros(40, width, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = gen(4)(40, 4, 64).to(F16)
+    good = ob.CacheBatch(i32(*range(41)), i32(*[300] * 40), wide, hint)
+    want = ob.cache_attend(q, cache, good)
+    assert status_ok()
+    starts_ = list(range(41))
+    starts_[7] = 3                                              # sequence 6 runs from 6 back to 3, sequence 7 from 3 to 8
+    ob.cache_attend(q, cache, ob.CacheBatch(i32(*starts_), good.kv_len, wide, hint))
+    assert not status_ok() and status_ok()
+    assert torch.equal(ob.cache_attend(q, cache, good), want)
+
+
 def test_outputs_that_overlap_are_refused():
     n = gen(9)
     x, w, r = n(8, 64).to(F16), n(64).to(F16), n(8, 64).to(F16)

@@ -100,7 +100,9 @@ __device__ __forceinline__ float scale_for(float amax) {
 
 // ---- programmatic dependent launch -----------------------------------------------------------------------------------------
 // A decode step is a chain of kernels of a few microseconds. They are launched so that a grid may start while its
-// predecessor drains, and each waits here, before its first access to memory, until the predecessor is complete.
+// predecessor drains, and each waits here, before its first access to memory, until the predecessor is complete. What a
+// predecessor may have written (lengths, tables, scales, tokens) is read by plain loads only: a read-only load (ld.global.nc)
+// promises that nothing writes the data while the kernel lives, and could be moved above the wait.
 __device__ __forceinline__ void follow_previous_kernel() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");

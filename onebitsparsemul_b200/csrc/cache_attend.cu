@@ -63,9 +63,9 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 __device__ __forceinline__ Seq seq_info(const ob::CacheAttendCall& c, int group, int s, int rows_per_tile) {
   Seq q;
-  const int q1 = __ldg(c.q_start + s + 1);
-  q.q0 = __ldg(c.q_start + s);
-  q.kv = __ldg(c.kv_len + s);
+  const int q1 = c.q_start[s + 1];
+  q.q0 = c.q_start[s];
+  q.kv = c.kv_len[s];
   q.bad = q.q0 < 0 || q1 > c.tokens || q1 < q.q0;
   q.n = q.bad || (int64_t)(q1 - q.q0) * group > c.few_rows ? 0 : q1 - q.q0;
   const int64_t room = c.table_width * kPageTokens;
@@ -162,7 +162,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     const int unit = blockIdx.x / ws.cluster, pair = unit / ws.tiles;
     page0 = blockIdx.x % ws.cluster, tile = unit % ws.tiles, head = pair % H, seq = pair / H;
     const int p = page0 + stride * (warp + kWarps * lane);      // the first page numbers do not wait for the lengths
-    if (p < c.table_width) first_id = __ldg(c.table + (int64_t)seq * c.table_stride + p);
+    if (p < c.table_width) first_id = c.table[(int64_t)seq * c.table_stride + p];
     q = seq_info(c, group, seq, kRows);
     if (q.bad && page0 == 0 && tile == 0 && head == 0 && threadIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
     if (tile >= q.tiles) return;                                // the whole cluster
@@ -232,13 +232,13 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     if constexpr (!LINE) {
       const int pg = page0 + stride * (warp + kWarps * (first + lane));
       if (first + lane < my_pages && (int64_t)pg * kPageTokens < q.kv) {
-        const int id = first == 0 ? first_id : __ldg(c.table + (int64_t)seq * c.table_stride + pg);
+        const int id = first == 0 ? first_id : c.table[(int64_t)seq * c.table_stride + pg];
         if (id < 0 || id >= c.pages) {
           atomicCAS(&g_attend_status, 0, kStatusBadBatch);
         } else {
           ph = (int64_t)id * H + head;
-          ph_ks = __ldg(c.k_scale + ph);
-          ph_vs = __ldg(c.v_scale + ph);
+          ph_ks = c.k_scale[ph];
+          ph_vs = c.v_scale[ph];
         }
       }
       return;
@@ -249,13 +249,13 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
       const int64_t seg = quotient(o, q.pages);
       const int pg = (int)(o - seg * q.pages), head = (int)quotient(seg, q.tiles);
       if ((int64_t)pg * kPageTokens < q.kv) {
-        const int id = __ldg(c.table + (int64_t)s * c.table_stride + pg);
+        const int id = c.table[(int64_t)s * c.table_stride + pg];
         if (id < 0 || id >= c.pages) {
           atomicCAS(&g_attend_status, 0, kStatusBadBatch);
         } else {
           ph = (int64_t)id * H + head;
-          ph_ks = __ldg(c.k_scale + ph);
-          ph_vs = __ldg(c.v_scale + ph);
+          ph_ks = c.k_scale[ph];
+          ph_vs = c.v_scale[ph];
         }
       }
     }

@@ -526,9 +526,9 @@ template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_jo
   if (row >= rows) return;
   const int t = (int)(row / c.heads);
   int first = 0;
-  for (int s0 = 0; s0 <= c.seqs; s0 += 32) first += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && __ldg(c.q_start + min((int64_t)s0 + lane, c.seqs)) <= t));
+  for (int s0 = 0; s0 <= c.seqs; s0 += 32) first += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && c.q_start[min((int64_t)s0 + lane, c.seqs)] <= t));
   if (first < 1 || first > c.seqs) return;                      // padding: not written
-  const int q0 = __ldg(c.q_start + first - 1), q1 = __ldg(c.q_start + first);
+  const int q0 = c.q_start[first - 1], q1 = c.q_start[first];
   if (q0 < 0 || q1 > c.tokens || (q1 - q0) * (c.heads / c.kv_heads) <= c.few_rows) return;
   const float* p = partial + row * (D + 4);
   const int64_t step = rows * (D + 4);

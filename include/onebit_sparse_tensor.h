@@ -256,10 +256,10 @@ int onebit_cache_attend(const void *q, int64_t q_token_stride, int64_t q_head_st
                         int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_new, float scale,
                         int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Synchronises the current device, then reads and clears its status word: ONEBIT_ERR_DEVICE_WAIT if
- * a bounded wait inside the tensor-memory kernel gave up since the last call (the kernel then still
- * terminated, with an unusable result), ONEBIT_ERR_BATCH if a cache operator left out a page or rows that a batch named
- * outside their range, ONEBIT_OK otherwise. The reference has no counterpart; its
+/* Synchronises the current device, then reads and clears its status words: ONEBIT_ERR_DEVICE_WAIT if
+ * a bounded wait inside a kernel gave up since the last call (the kernel then still
+ * terminated, with an unusable result), else ONEBIT_ERR_BATCH if a cache operator left out a page or rows that a batch named
+ * outside their range, else ONEBIT_OK; onebit_last_error says which kernel. The reference has no counterpart; its
  * kernel has no device-side waits on other agents. */
 int onebit_check_device_status(void);
 

@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "../../include/onebit_sparse_tensor.h"
+#include "device_status.h"
 #include "formats.h"
 #include "kernels.h"
 
@@ -335,9 +336,6 @@ int onebit_unpack_to_dense(const void* bits_tile, const void* meta_tile, const v
 
 // ---- the operators between the linear layers of a decoder block ----------------------------------------------------------
 namespace {
-// codes below this one are bounded waits that gave up; see block_common.h
-constexpr int kStatusBadBatch = 64;
-
 int check_type(int dtype) {
   return dtype == OB_DENSE_F16 || dtype == OB_DENSE_BF16 ? ONEBIT_OK : fail(ONEBIT_ERR_ARG, "unknown 16-bit type %d", dtype);
 }
@@ -448,35 +446,24 @@ int onebit_cache_attend(const void* q, int64_t q_token_stride, int64_t q_head_st
   return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "cache attention launch");
 }
 
-// Reads and clears the status words of the tensor-memory and decode kernels on the current device. Synchronises
-// the device. Returns ONEBIT_ERR_DEVICE_WAIT if a bounded wait inside a kernel gave up since the
-// last call.
+// Reads and clears every status word of the current device. Synchronises the device.
 int onebit_check_device_status(void) {
   int* status = nullptr;
   if (int rc = get_status_word(&status)) return rc;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize");
-  int host = 0;
-  e = cudaMemcpy(&host, status, sizeof(int), cudaMemcpyDeviceToHost);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpy(status)");
-  if (host != 0) {
-    cudaMemset(status, 0, sizeof(int));
-    return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the tensor-memory kernel gave up (role code %d)", host);
-  }
-  e = ob::read_decode_status(&host);
-  if (e != cudaSuccess) return cuda_fail(e, "read_decode_status");
-  if (host != 0) return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the decode kernel gave up (code %d)", host);
-  e = ob::read_fewtok_status(&host);
-  if (e != cudaSuccess) return cuda_fail(e, "read_fewtok_status");
-  if (host != 0) return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the few-token kernel gave up (code %d)", host);
-  e = ob::read_append_status(&host);
-  if (e != cudaSuccess) return cuda_fail(e, "read_append_status");
-  if (host != 0) return fail(ONEBIT_ERR_BATCH, "cache append: a page number or a sequence offset is outside its range (that page was not written)");
-  e = ob::read_attend_status(&host);
-  if (e != cudaSuccess) return cuda_fail(e, "read_attend_status");
-  if (host >= kStatusBadBatch) return fail(ONEBIT_ERR_BATCH, "cache attention: a page number or a sequence offset is outside its range (those tokens were left out)");
-  if (host != 0) return fail(ONEBIT_ERR_DEVICE_WAIT, "a bounded wait inside the cache attention kernel gave up (code %d)", host);
-  return ONEBIT_OK;
+  ob::DeviceStatus s;
+  e = cudaMemcpy(&s.tensor_memory_wait, status, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && s.tensor_memory_wait != 0) e = cudaMemset(status, 0, sizeof(int));
+  if (e != cudaSuccess) return cuda_fail(e, "status word of the tensor-memory kernel");
+  if ((e = ob::read_decode_status(&s.decode_wait)) != cudaSuccess) return cuda_fail(e, "read_decode_status");
+  if ((e = ob::read_fewtok_status(&s.few_token_wait)) != cudaSuccess) return cuda_fail(e, "read_fewtok_status");
+  if ((e = ob::read_append_status(&s.append_batch)) != cudaSuccess) return cuda_fail(e, "read_append_status");
+  if ((e = ob::read_attend_status(&s.attend_wait, &s.attend_batch)) != cudaSuccess) return cuda_fail(e, "read_attend_status");
+  if ((e = ob::read_attend_many_status(&s.attend_many_wait, &s.attend_many_batch)) != cudaSuccess) return cuda_fail(e, "read_attend_many_status");
+  char text[384];
+  const int rc = ob::describe(s, text, sizeof(text));
+  return rc == ONEBIT_OK ? rc : fail(rc, "%s", text);
 }
 
 }  // extern "C"

@@ -16,8 +16,17 @@ constexpr int kPageTokens = 64;
 constexpr float kE4m3Max = 448.f;
 constexpr int kMinScaleExp = -32, kMaxScaleExp = 32;
 
-// codes of the block kernels' status words
-constexpr int kStatusBadBatch = 64;   // a page number or a sequence offset outside its range: that work was skipped
+// Notes that a batch named a page or a range outside its tensors; what it named was left out. The word is apart from the one that
+// bounded waits leave their code in.
+__device__ __forceinline__ void note_bad_batch(int* word) { atomicExch(word, 1); }
+// A status word's value, and 0 in its place.
+template <typename Word> cudaError_t take_status(Word& symbol, int* out) {
+  *out = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(out, symbol, sizeof(int));
+  if (e != cudaSuccess || *out == 0) return e;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(symbol, &zero, sizeof(int));
+}
 
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

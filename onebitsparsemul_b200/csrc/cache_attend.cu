@@ -39,7 +39,7 @@ namespace {
 using namespace ob_block;
 using namespace ob_ptx;
 
-__device__ int g_attend_status;
+__device__ int g_attend_status, g_attend_batch;   // code of a wait that gave up; see note_bad_batch
 
 constexpr int kWarps = 4;
 constexpr int kRingBytes = 24 * 1024;             // per warp
@@ -164,7 +164,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     const int p = page0 + stride * (warp + kWarps * lane);      // the first page numbers do not wait for the lengths
     if (p < c.table_width) first_id = c.table[(int64_t)seq * c.table_stride + p];
     q = seq_info(c, group, seq, kRows);
-    if (q.bad && page0 == 0 && tile == 0 && head == 0 && threadIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+    if (q.bad && page0 == 0 && tile == 0 && head == 0 && threadIdx.x == 0) note_bad_batch(&g_attend_batch);
     if (tile >= q.tiles) return;                                // the whole cluster
     b = (q.tiles - tile + ws.tiles - 1) / ws.tiles;             // more than one round where the caller's bound was wrong
     take = q.pages > page0 ? (q.pages - page0 + stride - 1) / stride : 0;
@@ -184,7 +184,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
     mine += q.w;
     bad |= q.bad;
   }
-  if (bad && blockIdx.x == 0) atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+  if (bad && blockIdx.x == 0) note_bad_batch(&g_attend_batch);
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -234,7 +234,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
       if (first + lane < my_pages && (int64_t)pg * kPageTokens < q.kv) {
         const int id = first == 0 ? first_id : c.table[(int64_t)seq * c.table_stride + pg];
         if (id < 0 || id >= c.pages) {
-          atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+          note_bad_batch(&g_attend_batch);
         } else {
           ph = (int64_t)id * H + head;
           ph_ks = c.k_scale[ph];
@@ -251,7 +251,7 @@ ob_attend_few_kernel(const ob::CacheAttendCall c, const FewLayout ws) {
       if ((int64_t)pg * kPageTokens < q.kv) {
         const int id = c.table[(int64_t)s * c.table_stride + pg];
         if (id < 0 || id >= c.pages) {
-          atomicCAS(&g_attend_status, 0, kStatusBadBatch);
+          note_bad_batch(&g_attend_batch);
         } else {
           ph = (int64_t)id * H + head;
           ph_ks = c.k_scale[ph];
@@ -795,14 +795,9 @@ cudaError_t launch_cache_attend(const CacheAttendCall& call, void* workspace, cu
   return launch_cache_attend_many(c, workspace, stream);
 }
 
-cudaError_t read_attend_status(int* out) {
-  int few = 0;
-  cudaError_t e = read_attend_many_status(out);                 // a batch may have been both kernels'
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&few, g_attend_status, sizeof(int));
-  if (e != cudaSuccess || few == 0) return e;
-  *out = few;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_attend_status, &zero, sizeof(int));
+cudaError_t read_attend_status(int* wait, int* batch) {
+  const cudaError_t e = take_status(g_attend_status, wait);
+  return e == cudaSuccess ? take_status(g_attend_batch, batch) : e;
 }
 
 }  // namespace ob

@@ -10,7 +10,6 @@ namespace ob {
 // many query rows per cache head (cache_attend_sm100.cu)
 int64_t cache_attend_many_workspace(const CacheAttendCall& c);
 cudaError_t launch_cache_attend_many(const CacheAttendCall& c, void* workspace, cudaStream_t stream);
-cudaError_t read_attend_many_status(int* out);
 
 }  // namespace ob
 

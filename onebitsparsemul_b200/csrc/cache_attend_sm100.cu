@@ -35,7 +35,7 @@ namespace {
 using namespace ob_block;
 using namespace ob_ptx;
 
-__device__ int g_attend_many_status;
+__device__ int g_attend_many_status, g_attend_many_batch;       // code of a wait that gave up; see note_bad_batch
 
 constexpr int kTileRows = 128, kCtaRows = 256, kTileTokens = 128;
 constexpr int kProducers = 7;                                   // warps
@@ -149,14 +149,14 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   const int q0 = __ldg(c.q_start + seq), q1 = __ldg(c.q_start + seq + 1), kv_raw = __ldg(c.kv_len + seq);
   const int tile = slot - first_slot(seq);
   if (q0 < 0 || q1 > c.tokens || q1 < q0) {
-    if (threadIdx.x == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+    if (threadIdx.x == 0) note_bad_batch(&g_attend_many_batch);
     return;
   }
   const int n = q1 - q0, rows_all = n * group, row0 = tile * kCtaRows;
   if (rows_all <= c.few_rows) return;                           // cache_attend.cu's
   if (tile < 0 || row0 >= rows_all) return;                     // tile < 0: q_start runs backwards
   const int kv = (int)min((int64_t)max(kv_raw, 0), c.table_width * kPageTokens);
-  if (kv < kv_raw && threadIdx.x == 0) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+  if (kv < kv_raw && threadIdx.x == 0) note_bad_batch(&g_attend_many_batch);
   auto limit_of = [&](int r) { return c.causal ? min(kv, kv_raw - n + r / group + 1) : kv; };
   const int hi = max(0, limit_of(min(rows_all, row0 + kCtaRows) - 1));
   const int steps_all = (hi + kTileTokens - 1) / kTileTokens;
@@ -463,7 +463,7 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
       for (int values = 0; values < 2; ++values) {
         const int item = 2 * j + values, slot = item % C::kSlots;
         if (!held(now[0]) || !held(now[1])) {
-          if ((!held(now[0]) && now[0] != -2) || (!held(now[1]) && now[1] != -2)) atomicCAS(&g_attend_many_status, 0, kStatusBadBatch);
+          if ((!held(now[0]) && now[0] != -2) || (!held(now[1]) && now[1] != -2)) note_bad_batch(&g_attend_many_batch);
 #pragma unroll
           for (int i = 0; i < kTurns; ++i)
             if (!held(i * kProducers + pw < kUnits / 2 ? now[0] : now[1])) x[values][i] = make_uint4(0, 0, 0, 0);
@@ -594,11 +594,9 @@ cudaError_t launch_cache_attend_many(const CacheAttendCall& c, void* workspace, 
   return c.head_dim == 64 ? launch_many<__half, 64>(c, workspace, stream) : launch_many<__half, 128>(c, workspace, stream);
 }
 
-cudaError_t read_attend_many_status(int* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_attend_many_status, sizeof(int));
-  if (e != cudaSuccess || *out == 0) return e;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_attend_many_status, &zero, sizeof(int));
+cudaError_t read_attend_many_status(int* wait, int* batch) {
+  const cudaError_t e = take_status(g_attend_many_status, wait);
+  return e == cudaSuccess ? take_status(g_attend_many_batch, batch) : e;
 }
 
 }  // namespace ob

@@ -85,7 +85,7 @@ struct CacheAppendCall {
   bool bf16;
 };
 cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream);
-cudaError_t read_append_status(int* out);
+cudaError_t read_append_status(int* batch);           // the readers clear the words
 // attention over the cache (cache_attend.cu)
 struct CacheAttendCall {
   const void* q;
@@ -103,6 +103,7 @@ struct CacheAttendCall {
 };
 int64_t cache_attend_workspace(const CacheAttendCall& c);
 cudaError_t launch_cache_attend(const CacheAttendCall& c, void* workspace, cudaStream_t stream);
-cudaError_t read_attend_status(int* out);
+cudaError_t read_attend_status(int* wait, int* batch);
+cudaError_t read_attend_many_status(int* wait, int* batch);
 
 }  // namespace ob

@@ -22,7 +22,7 @@ namespace {
 
 using namespace ob_block;
 
-__device__ int g_append_status;
+__device__ int g_append_batch;   // see note_bad_batch
 
 struct Rotation {
   const double* freq;          // rotary_dim / 2 angular frequencies
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
   if (n <= 0 || kv <= 0) return;
   if (q0 < 0 || q1 > a.tokens) {
-    if (tid == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
+    if (tid == 0) note_bad_batch(&g_append_batch);
     return;
   }
   const int before = kv - n;                                  // may be negative: the first -before tokens have no place
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
     const int base = (int)block * kPageTokens;
     const int page = block < b.table_width ? b.table[(int64_t)seq * b.table_stride + block] : -1;
     if (page < 0 || page >= a.pages) {
-      if (tid == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
+      if (tid == 0) note_bad_batch(&g_append_batch);
       continue;
     }
     const int lo = max(before - base, 0), hi = min(kv - base, kPageTokens);      // places of the new tokens in the page
@@ -539,7 +539,7 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
   if (n <= 0 || kv <= 0) return;
   if (q0 < 0 || q1 > a.tokens) {
-    if (lane == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
+    if (lane == 0) note_bad_batch(&g_append_batch);
     return;
   }
   const int before = kv - n, mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + 1 - q0 / kPageTokens;
@@ -549,7 +549,7 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
     const int base = (int)block * kPageTokens;
     const int page = block < b.table_width ? b.table[(int64_t)seq * b.table_stride + block] : -1;
     if (page < 0 || page >= a.pages) {
-      if (lane == 0) atomicCAS(&g_append_status, 0, kStatusBadBatch);
+      if (lane == 0) note_bad_batch(&g_append_batch);
       continue;
     }
     const int lo = max(before - base, 0), hi = min(kv - base, kPageTokens);
@@ -674,11 +674,6 @@ cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream) {
   return c.bf16 ? by_dim(__nv_bfloat16{}) : by_dim(__half{});
 }
 
-cudaError_t read_append_status(int* out) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_append_status, sizeof(int));
-  if (e != cudaSuccess || *out == 0) return e;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(g_append_status, &zero, sizeof(int));
-}
+cudaError_t read_append_status(int* batch) { return take_status(g_append_batch, batch); }
 
 }  // namespace ob

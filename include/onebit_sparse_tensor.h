@@ -226,9 +226,10 @@ int onebit_rotary(const void *x, int64_t x_token_stride, int64_t x_head_stride, 
  * head_dim, 64), both e4m3 bytes, 16-byte aligned; k_scale, v_scale (pages, kv_heads) fp32: a stored value stands for
  * code * scale. head_dim 64 or 128. A batch (device int32): sequence s has the new tokens q_start[s] .. q_start[s+1] - 1 of the
  * call's `tokens` rows and kv_len[s] tokens in the cache INCLUDING the new ones; the token at position p lies in page
- * block_table[s * table_stride + p / 64]. Rows that belong to no sequence are neither read nor written. A page number outside
- * [0, pages), a position beyond table_width pages or rows beyond `tokens` are skipped, and onebit_check_device_status
- * reports ONEBIT_ERR_BATCH.
+ * block_table[s * table_stride + p / 64]. Rows that belong to no sequence are not written, and what they hold does not matter. A
+ * page number outside [0, pages) or a position beyond table_width pages is skipped; so is a sequence whose range is not inside the
+ * call's rows or runs backwards (where ranges overlap, rows that two sequences claim may be either's, or be skipped). The other
+ * sequences are not touched by that, and onebit_check_device_status reports ONEBIT_ERR_BATCH.
  *
  * onebit_cache_append turns k (as onebit_rotary at the tokens' own positions; rotary_dim 0: not at all) and stores k and v:
  * the page's scale becomes the smallest power of two from 2^-32 to 2^32 that brings the new tokens' largest finite |value| to

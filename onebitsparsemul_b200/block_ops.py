@@ -142,13 +142,14 @@ class CacheBatch:
 
         q_start      (sequences + 1,)  rows q_start[s] .. q_start[s + 1] of the step's tokens belong to sequence s
         kv_len       (sequences,)      tokens of the sequence in the cache, the new ones included
-        block_table  (sequences, width) page of each 64 tokens; entries behind a sequence's length are never read
+        block_table  (sequences, width) page of each 64 tokens; entries behind a sequence's length do not matter
 
     max_new: an upper bound of the sequences' new tokens, if the caller knows one (a decode step: 1). It picks the
     kernel, as the table's width does (the narrower, the better short batches are dealt out); results are right whatever it
-    says, though sums may be taken in another order. Rows outside q_start's range are padding: not read, and their outputs not written. The
-    values stay on the device and may be rewritten between steps (a captured step reads them anew). A page number or a range
-    that lies outside its tensor is left out, and ``onebit_check_device_status`` reports it."""
+    says, though sums may be taken in another order. Rows outside q_start's range are padding: what they hold does not matter, and their
+    outputs are not written. The values stay on the device and may be rewritten between steps (a captured step reads them anew). A page
+    number that lies outside its tensor is left out, and so is a sequence whose range does or that runs backwards;
+    the other sequences are not touched by that, and ``onebit_check_device_status`` reports it."""
 
     __slots__ = ("q_start", "kv_len", "block_table", "max_new", "seqs", "width")
 

@@ -72,6 +72,36 @@ template <> __device__ __forceinline__ void store8<float>(float* p, const float 
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// ---- whose rows these are --------------------------------------------------------------------------------------------------
+// A batch's q_start has to ascend from 0 or more to the call's rows or less. Where it does not, the batch is reported, and a sequence
+// is left out if its range is not inside the rows, runs backwards, or starts before an earlier start. For that the work is dealt
+// out by the running maximum Q[s] of the starts that lie in range: it ascends whatever q_start holds, and equals q_start for every
+// sequence that is not left out. Row t belongs to sequence s with Q[s] <= t < Q[s + 1]; slot x of a grid that gives sequence s the
+// slots Q[s] / per + s .. Q[s + 1] / per + s belongs to the last s with Q[s] / per + s <= x. Either is found by one minimum
+// over all starts, without the running maximum itself: the first s that is too far for a start q[i], i <= s.
+struct Starts {
+  const int* q;
+  int seqs, rows;
+  __device__ __forceinline__ bool in_range(int start) const { return start >= 0 && start <= rows; }
+  // start i, and whether it is out of order with the next one
+  __device__ __forceinline__ int at(int i, bool& bad) const {
+    const int a = q[i], b = i < seqs ? q[i + 1] : rows;
+    bad |= a < 0 || b < a || b > rows;
+    return a;
+  }
+  __device__ __forceinline__ int behind_row(int i, int start, int row) const { return in_range(start) && start > row ? i : seqs + 1; }
+  // place: start -> its share of the slot number
+  __device__ __forceinline__ int behind_slot(int i, int start, int slot, int place) const { return in_range(start) ? max(i, slot - place + 1) : seqs; }
+  // sequence s of a batch that is out of order; a walk over the starts before it, which a batch in order never takes
+  __device__ __forceinline__ bool left_out(int s) const {
+    const int a = q[s], b = q[s + 1];
+    if (a < 0 || b < a || b > rows) return true;
+    for (int i = 0; i < s; ++i)
+      if (in_range(q[i]) && q[i] > a) return true;
+    return false;
+  }
+};
+
 // ---- rotary angles -----------------------------------------------------------------------------------------------------
 // An angle is kept in turns, as a 64-bit binary fraction: the frequency's share of a turn per position, rounded to 2^-64
 // (from a double: 53 bits of it are meaningful), times the position, modulo 2^64 -- the integer product wraps exactly where

@@ -135,26 +135,30 @@ ob_attend_many_kernel(const ob::CacheAttendCall c, float* partial, int splits) {
   // ---- which rows: sequence s owns the row tiles [floor(q_start[s] group / 256) + s, the same of s + 1) of the grid ----
   const int slots = gridDim.x / H;
   const int head = blockIdx.x % H, slot = slots - 1 - (int)(blockIdx.x / H);     // the long causal tiles first
-  auto first_slot = [&](int s) { return (int)((int64_t)__ldg(c.q_start + s) * group / kCtaRows) + s; };
-  if (threadIdx.x == 0) found = 0;
+  const Starts starts{c.q_start, (int)c.seqs, (int)c.tokens};
+  auto place = [&](int start) { return (int)((int64_t)start * group / kCtaRows); };
+  if (threadIdx.x == 0) found = min(starts.seqs, slot + 1);
   __syncthreads();
+  bool bad = false;
   {
-    int n = 0;
-    for (int s = threadIdx.x; s < c.seqs; s += kThreads) n += first_slot(s) <= slot;
-    if (n) atomicAdd(&found, n);
+    int n = starts.seqs;
+    for (int s = threadIdx.x; s < starts.seqs; s += kThreads) {
+      const int start = starts.at(s, bad);
+      n = min(n, starts.behind_slot(s, start, slot, place(start)));
+    }
+    n = __reduce_min_sync(~0u, n);
+    if (lane == 0) atomicMin(&found, n);
   }
-  __syncthreads();
+  bad = __syncthreads_or(bad);
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) note_bad_batch(&g_attend_many_batch);
   const int seq = found - 1;
   if (seq < 0) return;
+  if (bad && starts.left_out(seq)) return;
   const int q0 = __ldg(c.q_start + seq), q1 = __ldg(c.q_start + seq + 1), kv_raw = __ldg(c.kv_len + seq);
-  const int tile = slot - first_slot(seq);
-  if (q0 < 0 || q1 > c.tokens || q1 < q0) {
-    if (threadIdx.x == 0) note_bad_batch(&g_attend_many_batch);
-    return;
-  }
+  const int tile = slot - place(q0) - seq;
   const int n = q1 - q0, rows_all = n * group, row0 = tile * kCtaRows;
   if (rows_all <= c.few_rows) return;                           // cache_attend.cu's
-  if (tile < 0 || row0 >= rows_all) return;                     // tile < 0: q_start runs backwards
+  if (row0 >= rows_all) return;
   const int kv = (int)min((int64_t)max(kv_raw, 0), c.table_width * kPageTokens);
   if (kv < kv_raw && threadIdx.x == 0) note_bad_batch(&g_attend_many_batch);
   auto limit_of = [&](int r) { return c.causal ? min(kv, kv_raw - n + r / group + 1) : kv; };
@@ -525,11 +529,18 @@ template <typename T, int D> __global__ void __launch_bounds__(256) ob_attend_jo
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = c.tokens * c.heads;
   if (row >= rows) return;
   const int t = (int)(row / c.heads);
-  int first = 0;
-  for (int s0 = 0; s0 <= c.seqs; s0 += 32) first += __popc(__ballot_sync(~0u, s0 + lane <= c.seqs && c.q_start[min((int64_t)s0 + lane, c.seqs)] <= t));
+  const Starts starts{c.q_start, (int)c.seqs, (int)c.tokens};
+  int first = starts.seqs + 1;                                  // sequence first - 1 holds the token
+  bool bad = false;
+  for (int s = lane; s <= starts.seqs; s += 32) {
+    const int start = starts.at(s, bad);
+    first = min(first, starts.behind_row(s, start, t));
+  }
+  first = __reduce_min_sync(~0u, first);
   if (first < 1 || first > c.seqs) return;                      // padding: not written
+  if (__any_sync(~0u, bad) && starts.left_out(first - 1)) return;
   const int q0 = c.q_start[first - 1], q1 = c.q_start[first];
-  if (q0 < 0 || q1 > c.tokens || (q1 - q0) * (c.heads / c.kv_heads) <= c.few_rows) return;
+  if ((q1 - q0) * (c.heads / c.kv_heads) <= c.few_rows) return;
   const float* p = partial + row * (D + 4);
   const int64_t step = rows * (D + 4);
   float M = -INFINITY;

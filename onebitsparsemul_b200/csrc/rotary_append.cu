@@ -188,16 +188,6 @@ template <typename T, int W, int TOKENS> __global__ void __launch_bounds__(kRotT
   });
 }
 
-// Number of sequences s with key(s) <= x, counted by the whole CTA (keys do not decrease with s).
-template <int THREADS, typename F> __device__ __forceinline__ int count_not_above(int seqs, int x, F key) {
-  int c = 0;
-  for (int s0 = 0; s0 < seqs; s0 += THREADS) {
-    const int s = s0 + threadIdx.x;
-    c += __syncthreads_count(s < seqs && key(s) <= x);
-  }
-  return c;
-}
-
 __device__ __forceinline__ float finite_max(float m, float v) {
   v = fabsf(v);
   return v <= 3.402823466e38f ? fmaxf(m, v) : m;
@@ -235,8 +225,10 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
   __shared__ __align__(16) float2 cs[kPageTokens][D / 2];
   __shared__ float red[2][kThreads / 32];
   __shared__ int nan_token[kPageTokens];
+  __shared__ int found[kThreads / 32][kAppendTokens];
   const int tid = threadIdx.x;
   const BatchArgs& b = a.b;
+  const Starts starts{b.q_start, b.seqs, a.tokens};
 
   // the CTAs of pages come first: they are the longer ones
   const int items = a.page_slots * a.kv_heads;
@@ -248,18 +240,27 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
     __shared__ bool skip[kAppendTokens];
     const int t0 = ((int)blockIdx.x - items) * kAppendTokens, n = min(kAppendTokens, q.tokens - t0);
     rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip, [&] {
-      int c[kAppendTokens] = {};                                 // sequence c - 1 holds the token
-      for (int s0 = 0; s0 <= b.seqs; s0 += kThreads) {
-        const int s = s0 + tid, start = s <= b.seqs ? b.q_start[s] : 0x7fffffff;
+      int c[kAppendTokens];                                      // sequence c - 1 holds the token
+      bool bad = false;
 #pragma unroll
-        for (int tt = 0; tt < kAppendTokens; ++tt) c[tt] += __syncthreads_count(start <= t0 + tt);
+      for (int tt = 0; tt < kAppendTokens; ++tt) c[tt] = b.seqs + 1;
+      for (int s = tid; s <= b.seqs; s += kThreads) {
+        const int start = starts.at(s, bad);
+#pragma unroll
+        for (int tt = 0; tt < kAppendTokens; ++tt) c[tt] = min(c[tt], starts.behind_row(s, start, t0 + tt));
       }
 #pragma unroll
-      for (int tt = 0; tt < kAppendTokens; ++tt)
-        if (tid == tt && tt < n) {
-          skip[tt] = c[tt] < 1 || c[tt] > b.seqs;             // before the first or behind the last sequence
-          pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c[tt] - 1] - b.q_start[c[tt]] + t0 + tt;
-        }
+      for (int tt = 0; tt < kAppendTokens; ++tt) {
+        c[tt] = __reduce_min_sync(~0u, c[tt]);
+        if ((tid & 31) == 0) found[tid >> 5][tt] = c[tt];
+      }
+      bad = __syncthreads_or(bad);
+      if (tid < n) {
+        int c = found[0][tid];
+        for (int w = 1; w < kThreads / 32; ++w) c = min(c, found[w][tid]);
+        skip[tid] = c < 1 || c > b.seqs || (bad && starts.left_out(c - 1));     // before the first or behind the last sequence
+        pos[tid] = skip[tid] ? 0 : (int64_t)b.kv_len[c - 1] - b.q_start[c] + t0 + tid;
+      }
       __syncthreads();
       fill_cos_sin<kThreads>(q.rot, pos, n, qcs);
       __syncthreads();
@@ -271,18 +272,25 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
   // Sequence s owns the slots [floor(q_start[s] / 64) + s, floor(q_start[s+1] / 64) + s + 1): at least floor(n / 64) + 1. n tokens
   // touch at most one page more than that, which the first slot then takes too.
   const int head = (int)blockIdx.x % a.kv_heads, slot = (int)blockIdx.x / a.kv_heads;
-  auto first_slot = [&](int s) { return b.q_start[s] / kPageTokens + s; };
-  const int seq = count_not_above<kThreads>(b.seqs, slot, first_slot) - 1;
+  int c = min(b.seqs, slot + 1);                              // sequence c - 1 has the slot
+  bool bad = false;
+  for (int s = tid; s < b.seqs; s += kThreads) {
+    const int start = starts.at(s, bad);
+    c = min(c, starts.behind_slot(s, start, slot, start / kPageTokens));
+  }
+  c = __reduce_min_sync(~0u, c);
+  if ((tid & 31) == 0) found[tid >> 5][0] = c;
+  bad = __syncthreads_or(bad);
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) c = min(c, found[w][0]);
+  if (bad && blockIdx.x == 0 && tid == 0) note_bad_batch(&g_append_batch);
+  const int seq = c - 1;
   if (seq < 0) return;
+  if (bad && starts.left_out(seq)) return;
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
   if (n <= 0 || kv <= 0) return;
-  if (q0 < 0 || q1 > a.tokens) {
-    if (tid == 0) note_bad_batch(&g_append_batch);
-    return;
-  }
   const int before = kv - n;                                  // may be negative: the first -before tokens have no place
   const int mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + seq + 1 - (q0 / kPageTokens + seq);
-  if (mine < 0) return;                                       // q_start runs backwards
   const Rotation& r = a.rot;
   constexpr int kVecs = D / 8;
   const int quad = (tid & 7) + 8 * ((tid >> 5) / (kVecs / 4)); // a warp: 8 x 4 of the groups
@@ -508,20 +516,22 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
   const int lane = threadIdx.x & 31;
   const BatchArgs& b = a.b;
   const int page_ctas = (a.page_slots * a.kv_heads + 3) / 4;
-  // sequences s with key(s) <= x, counted by the warp
-  auto count = [&](int seqs, int x, auto key) {
-    int c = 0;
-    for (int s0 = 0; s0 < seqs; s0 += 32) c += __popc(__ballot_sync(~0u, s0 + lane < seqs && key(s0 + lane) <= x));
-    return c;
-  };
+  const Starts starts{b.q_start, b.seqs, a.tokens};
   if ((int)blockIdx.x >= page_ctas) {
     const int t0 = ((int)blockIdx.x - page_ctas) * kFewTokens, n = min(kFewTokens, q.tokens - t0);
     static_assert(kFewTokens == kThreads / 32, "a token per warp");
     rotate_tokens<T, W, kThreads>(q, t0, n, qcs, skip, [&] {
       const int tt = threadIdx.x >> 5;                        // a warp finds a token's sequence
-      const int c = count(b.seqs + 1, t0 + tt, [&](int s) { return b.q_start[s]; });
+      int c = b.seqs + 1;
+      bool bad = false;
+      for (int s = lane; s <= b.seqs; s += 32) {
+        const int start = starts.at(s, bad);
+        c = min(c, starts.behind_row(s, start, t0 + tt));
+      }
+      c = __reduce_min_sync(~0u, c);
+      bad = __any_sync(~0u, bad);
       if (lane == 0) {
-        skip[tt] = c < 1 || c > b.seqs;
+        skip[tt] = c < 1 || c > b.seqs || (bad && starts.left_out(c - 1));
         pos[tt] = skip[tt] ? 0 : (int64_t)b.kv_len[c - 1] - b.q_start[c] + t0 + tt;
       }
       __syncthreads();
@@ -534,16 +544,20 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
   const int item = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (item >= a.page_slots * a.kv_heads) return;
   const int head = item % a.kv_heads, slot = item / a.kv_heads;
-  const int seq = count(b.seqs, slot, [&](int s) { return b.q_start[s] / kPageTokens + s; }) - 1;
-  if (seq < 0) return;
+  int c = min(b.seqs, slot + 1);                              // sequence c - 1 has the slot
+  bool bad = false;
+  for (int s = lane; s < b.seqs; s += 32) {
+    const int start = starts.at(s, bad);
+    c = min(c, starts.behind_slot(s, start, slot, start / kPageTokens));
+  }
+  c = __reduce_min_sync(~0u, c);
+  bad = __any_sync(~0u, bad);
+  if (bad && item == 0 && lane == 0) note_bad_batch(&g_append_batch);
+  const int seq = c - 1;
+  if (seq < 0 || (bad && starts.left_out(seq))) return;
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
   if (n <= 0 || kv <= 0) return;
-  if (q0 < 0 || q1 > a.tokens) {
-    if (lane == 0) note_bad_batch(&g_append_batch);
-    return;
-  }
   const int before = kv - n, mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + 1 - q0 / kPageTokens;
-  if (mine < 0) return;
   const Rotation& r = a.rot;
   for (int64_t block = max(before, 0) / kPageTokens + mine; block * kPageTokens < kv; block += slots) {
     const int base = (int)block * kPageTokens;

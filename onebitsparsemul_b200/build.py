@@ -73,17 +73,17 @@ def build_torch_extension(force: bool = False) -> str:
     root = os.path.dirname(HERE)
     srcs = [os.path.join(CSRC, f) for f in EXTENSION_SOURCES]
     out = os.path.join(root, "onebit_sparse_cuda" + sysconfig.get_config_var("EXT_SUFFIX"))
-    hdr = os.path.join(root, "include", "onebit_sparse_tensor.h")
+    hdrs = [os.path.join(root, "include", "onebit_sparse_tensor.h"), os.path.join(CSRC, "overlap.h")]
     objdir = os.path.join(HERE, "build")
     objs = [os.path.join(objdir, f.replace(".cpp", ".o")) for f in EXTENSION_SOURCES]
-    if not force and not _stale(out, [*srcs, hdr, lib]):
+    if not force and not _stale(out, [*srcs, *hdrs, lib]):
         return out
     inc = [f"-I{p}" for p in cpp_extension.include_paths("cuda")] + [f"-I{sysconfig.get_paths()['include']}",
                                                                   f"-I{os.path.join(root, 'include')}"]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=onebit_sparse_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc]
-    procs = [subprocess.Popen(["g++", *flags, "-c", src, "-o", obj]) for src, obj in zip(srcs, objs) if force or _stale(obj, [src, hdr])]
+    procs = [subprocess.Popen(["g++", *flags, "-c", src, "-o", obj]) for src, obj in zip(srcs, objs) if force or _stale(obj, [src, *hdrs])]
     if any([p.wait() for p in procs]):
         raise RuntimeError("g++ failed for onebit_sparse_cuda")
     subprocess.check_call(["g++", "-shared", *objs, "-o", out, f"-L{HERE}", "-lonebitmul", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_python",

@@ -2,7 +2,6 @@
 // the call into the C ABI of libonebitmul. The documented functions are those of onebitsparsemul_b200/block_ops.py, which
 // hand their arguments through: in a decode step these calls are a few microseconds of GPU work each, and checks and ctypes
 // conversions in Python took longer than that (a norm of one token: 21 us a call from Python through ctypes).
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -10,6 +9,7 @@
 #include <cmath>
 
 #include "onebit_sparse_tensor.h"
+#include "overlap.h"
 
 namespace {
 
@@ -48,11 +48,32 @@ int type_code(const Tensor& t) {
   return ONEBIT_DENSE_BF16;
 }
 
+ob_overlap::Place place_of(const Tensor& t) {
+  ob_overlap::Place p;
+  p.at = reinterpret_cast<uintptr_t>(t.data_ptr()), p.item = (int64_t)t.element_size();
+  if (t.is_contiguous()) {
+    p.add(p.item, t.numel());
+  } else if (t.dim() <= ob_overlap::kMaxDims) {
+    for (int64_t d = 0; d < t.dim(); ++d) p.add(t.stride(d) * (int64_t)t.element_size(), t.size(d));
+  } else {                                                      // the whole stretch
+    for (int64_t d = 0; d < t.dim(); ++d) p.item += t.stride(d) * (int64_t)t.element_size() * (t.size(d) - 1);
+  }
+  p.empty = t.numel() == 0;
+  return p;
+}
+// every value of one is the same value of the other
+bool is_same(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
 // An output has a place of its own for every value, and is an input as a whole or not at all.
 void check_output(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
-  TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, name, " has several values in one place");
+  const ob_overlap::Place place = place_of(out);
+  TORCH_CHECK_VALUE(!ob_overlap::may_overlap_itself(place), name, " has several values in one place");
   for (const Tensor* t : inputs)
-    TORCH_CHECK_VALUE(!t || at::get_overlap_status(out, *t) != at::MemOverlapStatus::Partial, name, " overlaps an input without being it");
+    TORCH_CHECK_VALUE(!t || is_same(out, *t) || !ob_overlap::may_overlap(place, place_of(*t)), name, " overlaps an input without being it");
 }
 
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -129,7 +150,6 @@ int rotary_dim_of(const Tensor& inv_freq, int64_t head_dim) {
 void check_turned(const Tensor& out, const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && (out.stride(2) == 1 || out.size(2) == 1), name,
                     " must have the input's shape and type and contiguous heads");
-  TORCH_CHECK_VALUE(out.data_ptr() != x.data_ptr() || out.strides() == x.strides(), name, " overlaps the input without being it");
   check_output(out, name, {&x});
 }
 
@@ -239,7 +259,7 @@ Tensor cache_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
   TORCH_CHECK_VALUE(!out || (out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->is_contiguous() && aligned(*out)),
                     "out must be contiguous (and 16-byte aligned) with q's shape and type");
-  TORCH_CHECK_VALUE(!out || at::get_overlap_status(*out, q) == at::MemOverlapStatus::No || at::get_overlap_status(*out, q) == at::MemOverlapStatus::TooHard, "out overlaps q");
+  TORCH_CHECK_VALUE(!out || !ob_overlap::may_overlap(place_of(*out), place_of(q)), "out overlaps q");
   Tensor y = out ? *out : torch::empty(q.sizes(), q.options());
   if (tokens > 0) {
     const bool as_it_is = q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && aligned(q);

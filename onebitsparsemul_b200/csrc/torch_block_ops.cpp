@@ -68,12 +68,14 @@ bool is_same(const Tensor& a, const Tensor& b) {
     if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
   return true;
 }
-// An output has a place of its own for every value, and is an input as a whole or not at all.
-void check_output(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs) {
+// An output has a place of its own for every value, and is an input as a whole or not at all; no part of it is an input that
+// other values are computed from (`apart`).
+void check_output(const Tensor& out, const char* name, std::initializer_list<const Tensor*> inputs, std::initializer_list<const Tensor*> apart = {}) {
   const ob_overlap::Place place = place_of(out);
   TORCH_CHECK_VALUE(!ob_overlap::may_overlap_itself(place), name, " has several values in one place");
   for (const Tensor* t : inputs)
     TORCH_CHECK_VALUE(!t || is_same(out, *t) || !ob_overlap::may_overlap(place, place_of(*t)), name, " overlaps an input without being it");
+  for (const Tensor* t : apart) TORCH_CHECK_VALUE(!t || !ob_overlap::may_overlap(place, place_of(*t)), name, " overlaps an input");
 }
 
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -147,10 +149,10 @@ int rotary_dim_of(const Tensor& inv_freq, int64_t head_dim) {
   TORCH_CHECK_VALUE(2 * inv_freq.numel() <= head_dim, inv_freq.numel(), " pairs do not fit a head of ", head_dim);
   return (int)(2 * inv_freq.numel());
 }
-void check_turned(const Tensor& out, const Tensor& x, const char* name) {
+void check_turned(const Tensor& out, const Tensor& x, const char* name, std::initializer_list<const Tensor*> apart) {
   TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && (out.stride(2) == 1 || out.size(2) == 1), name,
                     " must have the input's shape and type and contiguous heads");
-  check_output(out, name, {&x});
+  check_output(out, name, {&x}, apart);
 }
 
 Tensor rotary_tokens(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, const std::string& layout, double magnitude, const OptTensor& out_) {
@@ -165,7 +167,7 @@ Tensor rotary_tokens(const Tensor& x, const Tensor& positions, const Tensor& inv
   TORCH_CHECK_VALUE((wide || positions.scalar_type() == torch::kInt) && positions.dim() == 1 && positions.size(0) == tokens, "positions must be (tokens,) int32 or int64");
   const bool inter = interleaved_layout(layout);
   const int rotary_dim = rotary_dim_of(inv_freq, dim);
-  if (out) check_turned(*out, x, "out");
+  if (out) check_turned(*out, x, "out", {&positions, &inv_freq});
   Tensor y = out ? *out : torch::empty(x.sizes(), x.options());
   if (tokens > 0) {
     const Tensor x1 = inner_contiguous(x), p = positions.contiguous();
@@ -226,7 +228,7 @@ py::object cache_append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
     heads = q->size(1);
     TORCH_CHECK_VALUE(inv_freq, "q is only turned: it needs inv_freq");
     TORCH_CHECK_VALUE(heads % H == 0 && heads >= 1 && heads <= 4096, heads, " query heads are no multiple of ", H, " cache heads");
-    if (q_out) check_turned(*q_out, *q, "q_out");
+    if (q_out) check_turned(*q_out, *q, "q_out", {&k, &v, inv_freq, &k_pages, &v_pages, &k_scale, &v_scale, &q_start, &kv_len, &table});
     y = q_out ? *q_out : torch::empty(q->sizes(), q->options());
     q1 = inner_contiguous(*q);
   } else {
@@ -259,7 +261,7 @@ Tensor cache_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
   TORCH_CHECK_VALUE(!out || (out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->is_contiguous() && aligned(*out)),
                     "out must be contiguous (and 16-byte aligned) with q's shape and type");
-  TORCH_CHECK_VALUE(!out || !ob_overlap::may_overlap(place_of(*out), place_of(q)), "out overlaps q");
+  if (out) check_output(*out, "out", {}, {&q, &k_pages, &v_pages, &k_scale, &v_scale, &q_start, &kv_len, &table});
   Tensor y = out ? *out : torch::empty(q.sizes(), q.options());
   if (tokens > 0) {
     const bool as_it_is = q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && aligned(q);

@@ -59,3 +59,22 @@ def test_attention_views():
     for q, out in ((rows[:, :1], flat[:512].view(8, 1, 64)), (rows[:, 1:3], flat[128:128 + 1024].view(8, 2, 64))):
         with pytest.raises(ValueError):
             ob.cache_attend(q, cache, batch, out=out)
+
+
+def test_append_queries_apart_from_keys_values_and_cache():
+    """Queries are turned while other threads read k and v and write the pages: none of them may be where q_out is."""
+    cache = ob.KVCache8.empty(2, 4, 64)
+    batch = ob.CacheBatch(i32(0, 8), i32(8), i32(0).view(1, 1))
+    rows, freq = rows_of(8, 16), ob.rotary_frequencies(64)[0]
+    q, k, v = rows[:, :4], rows[:, 4:8], rows[:, 8:12]
+    pages = cache.k_pages.view(torch.uint8).view(-1)[: 8 * 4 * 64 * 2].view(F16).view(8, 4, 64)
+    for out in (k, v, rows[:, 5:9], rows[:, 3:7], rows[:, 11:15], pages):
+        with pytest.raises(ValueError):
+            ob.cache_append(k, v, cache, batch, q=q, inv_freq=freq, q_out=out)
+    before = rows.clone()
+    want = ob.cache_append(k, v, cache, batch, q=q, inv_freq=freq)
+    assert torch.equal(rows, before)
+    assert torch.equal(ob.cache_append(k, v, cache, batch, q=q, inv_freq=freq, q_out=rows[:, 12:]), want)
+    assert torch.equal(ob.cache_append(k, v, cache, batch, q=q, inv_freq=freq, q_out=q), want) and torch.equal(rows[:, 4:12], before[:, 4:12])
+    with pytest.raises(ValueError):
+        ob.cache_attend(q, cache, batch, out=pages)

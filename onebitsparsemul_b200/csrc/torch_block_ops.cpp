@@ -109,8 +109,9 @@ py::object residual_norm(const Tensor& x, const Tensor& weight, const OptTensor&
     h = residual_out ? *residual_out : torch::empty(x.sizes(), residual->options());
     r2 = rows_of(*residual, hidden);
   }
-  if (out) check_output(*out, "out", {&x, residual, gate, residual_out});
-  if (residual_out) check_output(*residual_out, "residual_out", {&x, residual, gate});
+  // the weights are read for every row, and weight after h is written
+  if (out) check_output(*out, "out", {&x, residual, gate, residual_out}, {&weight, post});
+  if (residual_out) check_output(*residual_out, "residual_out", {&x, residual, gate}, {&weight, post});
   TORCH_CHECK_VALUE(!out || !residual_out || out->numel() == 0 || out->data_ptr() != residual_out->data_ptr(), "out and residual_out must be different tensors");
   Tensor g2;
   int64_t gate_stride = 0;

@@ -78,3 +78,18 @@ def test_append_queries_apart_from_keys_values_and_cache():
     assert torch.equal(ob.cache_append(k, v, cache, batch, q=q, inv_freq=freq, q_out=q), want) and torch.equal(rows[:, 4:12], before[:, 4:12])
     with pytest.raises(ValueError):
         ob.cache_attend(q, cache, batch, out=pages)
+
+
+def test_norm_outputs_apart_from_the_weights():
+    """h is written before the weight is read: a residual_out that is the weight gave the norm a changed one."""
+    x, r, w, p = rows_of(1, 1, 96).view(1, 96), rows_of(1, 2, 96)[:, 1], rows_of(3, 1, 96)[:1].view(96).clone(), rows_of(4, 1, 96)[:1].view(96).clone()
+    many = rows_of(5, 1, 96).view(5, 96)
+    for kw in (dict(residual_out=w.view(1, 96)), dict(out=w.view(1, 96)), dict(residual_out=p.view(1, 96), post_weight=p), dict(out=p.view(1, 96), post_weight=p)):
+        with pytest.raises(ValueError):
+            ob.residual_norm(x, w, residual=r, **kw)
+    with pytest.raises(ValueError):
+        ob.residual_norm(many, many[2], out=many)
+    want = ob.residual_norm(x, w, residual=r, gate=p.view(1, 96))
+    gate = p.clone().view(1, 96)
+    got = ob.residual_norm(x, w, residual=r, gate=gate, residual_out=gate)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and got[1] is gate

@@ -193,6 +193,9 @@ std::tuple<int64_t, int64_t, int64_t> check_cache(const Tensor& k_pages, const T
   for (const Tensor* t : {&k_pages, &v_pages, &k_scale, &v_scale})
     TORCH_CHECK_VALUE(t->is_contiguous() && t->device() == k_pages.device(), "pages and scales must be contiguous, on one device");
   TORCH_CHECK_VALUE(pages >= 1 && heads >= 1 && heads <= 4096, "need at least one page and 1 to 4096 heads");
+  const ob_overlap::Place places[] = {place_of(k_pages), place_of(v_pages), place_of(k_scale), place_of(v_scale)};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j) TORCH_CHECK_VALUE(!ob_overlap::may_overlap(places[i], places[j]), "pages and scales must be four tensors that share no memory");
   return {pages, heads, dim};
 }
 

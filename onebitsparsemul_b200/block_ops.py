@@ -3,7 +3,7 @@ key/value cache and the attention that reads it. Every function is one call into
 kernels); the reference leaves these parts to the model it patches (tests/python/test_model_replace.py:22-44).
 
 Serving only, like the packed layers: no function records a gradient, and one that is handed a tensor that wants a
-gradient (with gradients enabled) refuses it. Tensors are float16 or bfloat16 on one CUDA device; work is queued on that
+gradient (with gradients enabled) or carries a forward-mode tangent refuses it. Tensors are float16 or bfloat16 on one CUDA device; work is queued on that
 device's current stream, nothing synchronises, and every call can be captured in a CUDA graph.
 
 The cache. `KVCache8` holds pages of 64 tokens: keys (pages, kv_heads, 64, head_dim), values transposed

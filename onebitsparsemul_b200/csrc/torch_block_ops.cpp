@@ -3,6 +3,7 @@
 // hand their arguments through: in a decode step these calls are a few microseconds of GPU work each, and checks and ctypes
 // conversions in Python took longer than that (a norm of one token: 21 us a call from Python through ctypes).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -31,15 +32,15 @@ void check_rc(int rc) {
   if (rc != ONEBIT_OK) raise_library_error("libonebitmul error " + std::to_string(rc) + ": " + onebit_last_error());
 }
 
-// every tensor on `device`, none of them waiting for a gradient
+// every tensor on `device`, none of them waiting for a gradient or with a forward-mode tangent
 void check_tensors(c10::Device device, std::initializer_list<const Tensor*> tensors) {
-  if (!device.is_cuda()) raise_library_error("no CUDA tensor: this library has no CPU path");
-  const bool grad = at::GradMode::is_enabled();
+  const bool grad = at::GradMode::is_enabled(), tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : tensors) {
-    if (!t) continue;
-    TORCH_CHECK_VALUE(t->device() == device, "tensors on different devices: ", t->device(), " and ", device);
-    TORCH_CHECK_VALUE(!grad || !t->requires_grad(), "a tensor wants a gradient, and this operator has none: call it under torch.no_grad()");
+    TORCH_CHECK_VALUE(!t || !grad || !t->requires_grad(), "a tensor wants a gradient, and this operator has none: call it under torch.no_grad()");
+    TORCH_CHECK_VALUE(!t || !tangents || !t->_fw_grad(0).defined(), "a tensor has a forward-mode tangent, and this operator has no derivative: give it the primal");
   }
+  if (!device.is_cuda()) raise_library_error("no CUDA tensor: this library has no CPU path");
+  for (const Tensor* t : tensors) TORCH_CHECK_VALUE(!t || t->device() == device, "tensors on different devices: ", t->device(), " and ", device);
 }
 
 int type_code(const Tensor& t) {
@@ -217,7 +218,7 @@ py::object cache_append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
                         const std::string& layout, double magnitude, const OptTensor& q_out_) {
   const Tensor *q = ptr(q_), *inv_freq = ptr(inv_freq_), *q_out = ptr(q_out_);
   const int code = type_code(k);
-  check_tensors(k.device(), {&k, &v, q, inv_freq, q_out, &k_pages, &table});
+  check_tensors(k.device(), {&k, &v, q, inv_freq, q_out, &k_pages, &k_scale, &v_scale, &table});
   const int64_t H = k_pages.size(1), D = k_pages.size(3), tokens = k.dim() == 3 ? k.size(0) : -1;
   check_heads(k, "k", -1, H, D);
   check_heads(v, "v", tokens, H, D);
@@ -254,7 +255,7 @@ Tensor cache_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
                     const Tensor& kv_len, const Tensor& table, int64_t max_new, const c10::optional<double>& scale_, bool causal, const OptTensor& out_) {
   const Tensor* out = ptr(out_);
   const int code = type_code(q);
-  check_tensors(q.device(), {&q, out, &k_pages, &table});
+  check_tensors(q.device(), {&q, out, &k_pages, &k_scale, &v_scale, &table});
   const int64_t H = k_pages.size(1), D = k_pages.size(3);
   check_heads(q, "q", -1, -1, D);
   const int64_t tokens = q.size(0), heads = q.size(1);

@@ -183,6 +183,14 @@ class CachedLlamaStack(nn.Module):
             for p in self.parameters():                          # N(0, 1 / fan_in): activations keep their scale
                 p.copy_((torch.randn(p.shape, generator=g) / p.shape[1] ** 0.5).to(p.dtype))
 
+    def _apply(self, fn, *args, **kw):
+        """`half()`, `to(dtype)` and the like: the frequencies move, but stay in 64 bits, which far positions need."""
+        freq = self.inv_freq
+        super()._apply(fn, *args, **kw)
+        if self.inv_freq.dtype != freq.dtype:
+            self.inv_freq = freq.to(self.inv_freq.device)
+        return self
+
     def make_caches(self, pages: int, device="cuda"):
         return [block_ops.KVCache8.empty(pages, self.kv_heads, self.head_dim, device=device) for _ in self.blocks]
 

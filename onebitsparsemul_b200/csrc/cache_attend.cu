@@ -710,6 +710,50 @@ int few_grid(const ob::CacheAttendCall& c) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(2 * ob::sm_count(), most));
 }
 
+constexpr int few_smem(int head_dim) { return kWarps * kRingBytes + kWarps * 8 * (head_dim + 4) * 4; }
+
+// The largest cluster, up to 16 CTAs, that the kernel of one type can be launched with on the current device.
+template <typename T, int D, int NT> int placeable() {
+  static std::atomic<uint64_t> ready{0};
+  if (allow_shared_memory(ob_attend_few_kernel<T, D, NT, false>, few_smem(D), ready, true) != cudaSuccess) {
+    cudaGetLastError();                                         // not a later launch's error
+    return 0;
+  }
+  for (int n = kMaxCluster; n >= 1; n /= 2) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)n, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)n), cfg.blockDim = dim3(kWarps * 32), cfg.dynamicSmemBytes = few_smem(D), cfg.attrs = &attr, cfg.numAttrs = 1;
+    int clusters = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, ob_attend_few_kernel<T, D, NT, false>, &cfg);
+    if (e != cudaSuccess) cudaGetLastError();
+    else if (clusters > 0) return n;
+  }
+  return 0;
+}
+// The same for both types of queries (the workspace is asked for without a type), looked up once per device. 0 without a device.
+int largest_cluster(int head_dim, int row_tiles) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  static std::atomic<int8_t> known[64][2][2];                   // largest + 1
+  std::atomic<int8_t>& k = known[dev & 63][head_dim == 128][row_tiles - 1];
+  if (const int v = k.load(std::memory_order_acquire)) return v - 1;
+  int n = 0;
+  auto of = [&](auto d, auto nt) { n = std::min(placeable<__half, decltype(d)::value, decltype(nt)::value>(), placeable<__nv_bfloat16, decltype(d)::value, decltype(nt)::value>()); };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Narrow = std::integral_constant<int, 64>;
+  using Wide = std::integral_constant<int, 128>;
+  if (head_dim == 128) row_tiles == 1 ? of(Wide{}, One{}) : of(Wide{}, Two{});
+  else row_tiles == 1 ? of(Narrow{}, One{}) : of(Narrow{}, Two{});
+  k.store((int8_t)(n + 1), std::memory_order_release);
+  return n;
+}
+
 // CTAs of a cluster per segment, 0: the line of pages. A cluster knows its segment from its number, asks for page numbers at
 // once and joins through shared memory: 1 token of 32 heads over 4096 tokens 9.7 us against 18.3 on the line (2.3 us from the
 // lengths to the first request saved, and the join kernel), 64 sequences of up to 1024 tokens 18.9 against 38 us (a CTA each;
@@ -717,19 +761,22 @@ int few_grid(const ob::CacheAttendCall& c) {
 // the rest of the batch is: 4 sequences of up to 32768 tokens 40-49 us, on the line 32-56. So it is taken where the block table's
 // width bounds the rounds: by 3 more than the line's if all sequences were as long, and for more than one sequence by 16, or 8
 // with several CTAs a segment. Clusters of 16 are slower than of 8 as soon as not all are resident (16 segments: 14.6 / 9.1 us).
+// What the device cannot place (largest_cluster) is not asked of it: the line needs no cluster.
 int few_cluster(const ob::CacheAttendCall& c) {
+  const int largest = largest_cluster((int)c.head_dim, few_tiles(c));
+  if (largest == 0) return 0;
   const int64_t segments = c.seqs * c.kv_heads * row_tiles(c), sms = ob::sm_count(), slots = 2 * sms, width = c.table_width;
   if (segments > 1 << 24) return 0;
   int n = 1;
-  while (n < 8 && segments * n * 2 <= slots && width > kMinPages * n) n *= 2;
-  if (n == 8 && segments * 16 <= sms && width > kMinPages * 8) n = 16;
+  while (n < 8 && n < largest && segments * n * 2 <= slots && width > kMinPages * n) n *= 2;
+  if (n == 8 && largest == 16 && segments * 16 <= sms && width > kMinPages * 8) n = 16;
   const int64_t rounds = (width + kWarps * n - 1) / (kWarps * n), line = segments * width / (kWarps * slots);
   return rounds <= line + 3 && (c.seqs == 1 || rounds <= (n == 1 ? 16 : 8)) ? n : 0;
 }
 
 template <typename T, int D, int NT> cudaError_t launch_few(const ob::CacheAttendCall& c, void* workspace, cudaStream_t stream) {
   const int grid = few_grid(c);
-  constexpr int smem = kWarps * kRingBytes + kWarps * 8 * (D + 4) * 4;
+  constexpr int smem = few_smem(D);
   const int64_t group = c.heads / c.kv_heads;
   FewLayout ws{(int)group, (uint64_t)(((1ll << 40) + group - 1) / group), static_cast<Header*>(workspace), 0, 0,
                reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ((grid * sizeof(Header) + 255) & ~size_t(255)))};

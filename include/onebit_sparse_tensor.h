@@ -243,6 +243,14 @@ int onebit_cache_append(const void *k, int64_t k_token_stride, int64_t k_head_st
                         float *k_scale, float *v_scale, int64_t pages, const int *q_start, const int *kv_len, const int *block_table,
                         int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
                         int64_t head_dim, int dtype, void *stream);
+/* The same with the caller's bound of a sequence's new tokens (0: tokens), as onebit_cache_attend has it: it only selects the
+ * kernels, results are right for any value. Without one, single tokens of many sequences take a launch more. */
+int onebit_cache_append_ex(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                           const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                           const double *inv_freq, int rotary_dim, int interleaved, float magnitude, void *k_pages, void *v_pages,
+                           float *k_scale, float *v_scale, int64_t pages, const int *q_start, const int *kv_len, const int *block_table,
+                           int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                           int64_t head_dim, int64_t max_new, int dtype, void *stream);
 
 /* out (tokens, heads, head_dim) = softmax(scale * q k^T) v over each sequence's cache; head h reads cache head
  * h / group, group = heads / kv_heads, tokens * group^2 < 2^40. causal: a new token at position p sees the positions up to p (the new tokens are the last of

@@ -42,6 +42,7 @@ SIGNATURES = {
     "onebit_residual_norm": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _f32, _f32, _int, _vp]),
     "onebit_rotary": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _int, _vp, _int, _int, _f32, _i64, _i64, _i64, _int, _vp]),
     "onebit_cache_append": (_int, [_vp, _i64, _i64] * 4 + [_vp, _int, _int, _f32] + [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] * 7 + [_int, _vp]),
+    "onebit_cache_append_ex": (_int, [_vp, _i64, _i64] * 4 + [_vp, _int, _int, _f32] + [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] * 8 + [_int, _vp]),
     "onebit_cache_attend_workspace": (_sz, [_i64] * 7),
     "onebit_cache_attend": (_int, [_vp, _i64, _i64] * 2 + [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] * 8 + [_f32, _int, _int, _vp, _sz, _vp]),
 }

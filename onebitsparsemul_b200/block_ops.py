@@ -145,7 +145,7 @@ class CacheBatch:
         block_table  (sequences, width) page of each 64 tokens; entries behind a sequence's length do not matter
 
     max_new: an upper bound of the sequences' new tokens, if the caller knows one (a decode step: 1). It picks the
-    kernel, as the table's width does (the narrower, the better short batches are dealt out); results are right whatever it
+    kernels of both, as the table's width does attention's (the narrower, the better short batches are dealt out); results are right whatever it
     says, though sums may be taken in another order. Rows outside q_start's range are padding: what they hold does not matter, and their
     outputs are not written. The values stay on the device and may be rewritten between steps (a captured step reads them anew). A page
     number that lies outside its tensor is left out, and so is a sequence whose range does or that runs backwards;
@@ -162,8 +162,8 @@ class CacheBatch:
 
 def cache_append(k, v, cache, batch, q=None, inv_freq=None, layout="half", magnitude=1.0, q_out=None):
     """Store the step's keys and values (tokens, kv_heads, head_dim) in the cache, keys turned by their positions if `inv_freq` is
-    given, and turn the queries q (tokens, heads, head_dim) too, all in one launch (``onebit_cache_append``). Returns the turned
-    queries (None without q); `q_out` may be q itself.
+    given, and turn the queries q (tokens, heads, head_dim) too, in one launch, or two where most sequences bring up to three tokens
+    and some more (``onebit_cache_append_ex``). Returns the turned queries (None without q); `q_out` may be q itself.
 
     The scale of a page and head is the smallest power of two (2^-32 to 2^32) that brings the largest finite |value| of its
     tokens into e4m3's range; when a step's tokens make it grow, the page's earlier tokens are re-scaled. Infinities are
@@ -171,7 +171,7 @@ def cache_append(k, v, cache, batch, q=None, inv_freq=None, layout="half", magni
     made NaN, so that the queries that see the token answer NaN and no others. A page that a step writes must belong to one
     sequence of the batch only."""
     return _ext().cache_append(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, batch.q_start, batch.kv_len, batch.block_table,
-                               q, inv_freq, layout, magnitude, q_out)
+                               batch.max_new, q, inv_freq, layout, magnitude, q_out)
 
 
 def cache_attend(q, cache, batch, scale=None, causal=True, out=None):

@@ -392,6 +392,17 @@ int onebit_cache_append(const void* k, int64_t k_token_stride, int64_t k_head_st
                         float* k_scale, float* v_scale, int64_t pages, const int* q_start, const int* kv_len, const int* block_table,
                         int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
                         int64_t head_dim, int dtype, void* stream) {
+  return onebit_cache_append_ex(k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, q, q_token_stride, q_head_stride, q_out,
+                                q_out_token_stride, q_out_head_stride, inv_freq, rotary_dim, interleaved, magnitude, k_pages, v_pages, k_scale, v_scale,
+                                pages, q_start, kv_len, block_table, table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim, 0, dtype, stream);
+}
+
+int onebit_cache_append_ex(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                           const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
+                           const double* inv_freq, int rotary_dim, int interleaved, float magnitude, void* k_pages, void* v_pages,
+                           float* k_scale, float* v_scale, int64_t pages, const int* q_start, const int* kv_len, const int* block_table,
+                           int64_t table_stride, int64_t table_width, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                           int64_t head_dim, int64_t max_new, int dtype, void* stream) {
   if (!k || !v || !k_pages || !v_pages || !k_scale || !v_scale || (q && !q_out)) return fail(ONEBIT_ERR_NULL, "null operand pointer");
   if (int rc = check_type(dtype)) return rc;
   if (int rc = check_batch(q_start, kv_len, block_table, table_width, tokens, seqs, q ? heads : kv_heads, kv_heads, head_dim, pages)) return rc;
@@ -400,7 +411,8 @@ int onebit_cache_append(const void* k, int64_t k_token_stride, int64_t k_head_st
   if (tokens == 0) return ONEBIT_OK;
   ob::CacheAppendCall c{k, v, q, q_out, k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride,
                         q_out_token_stride, q_out_head_stride, inv_freq, rotary_dim, interleaved != 0, magnitude, k_pages, v_pages, k_scale, v_scale,
-                        pages, q_start, kv_len, block_table, table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim, dtype == OB_DENSE_BF16};
+                        pages, q_start, kv_len, block_table, table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim, dtype == OB_DENSE_BF16,
+                        max_new > 0 && max_new < tokens ? max_new : tokens};
   cudaError_t e = ob::launch_cache_append(c, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? ONEBIT_OK : cuda_fail(e, "cache append launch");
 }

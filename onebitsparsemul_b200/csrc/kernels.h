@@ -83,6 +83,7 @@ struct CacheAppendCall {
   const int *q_start, *kv_len, *table;
   int64_t table_stride, table_width, tokens, seqs, heads, kv_heads, head_dim;
   bool bf16;
+  int64_t max_new;             // the caller's bound of a sequence's new tokens: it picks the kernels, results are right whatever it is
 };
 cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream);
 cudaError_t read_append_status(int* batch);           // the readers clear the words

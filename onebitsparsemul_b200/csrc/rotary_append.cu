@@ -60,6 +60,7 @@ struct AppendArgs {
   Rotation rot;                        // half = 0: keys are stored as they come
   int tokens;
   int page_slots;                      // CTAs of the append half of the grid: page slots x kv_heads
+  int least_new, most_new;             // this launch has the sequences with so many new tokens, least_new >= 1
 };
 
 constexpr int kAppendTokens = 4, kFewTokens = 4;   // query tokens per CTA of an append: with prompts, with steps
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
   if (seq < 0) return;
   if (bad && starts.left_out(seq)) return;
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
-  if (n <= 0 || kv <= 0) return;
+  if (n < a.least_new || n > a.most_new || kv <= 0) return;
   const int before = kv - n;                                  // may be negative: the first -before tokens have no place
   const int mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + seq + 1 - (q0 / kPageTokens + seq);
   const Rotation& r = a.rot;
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(2 * D, 768 / (2 * D)) ob_cache_append_kernel(c
 // The same for steps of few tokens (rotation of the queries included): a warp owns a page of a head, and everything is a rolled
 // loop over the page's new tokens and over 32 values at a time, twice -- for the largest value, then for the codes. The kernel
 // above takes 13.4 us for one token in each of 64 sequences, nearly all of it instruction fetches: a CTA runs its unrolled program
-// once. This one takes 6.2 us; with more tokens in a page the other is faster (the rule and its figures are in the launcher).
+// once. This one takes 5.8 us; with more tokens in a page the other is faster (the rule and its figures are in the launcher).
 template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_cache_append_few_kernel(const AppendArgs a, const RotaryArgs q) {
   follow_previous_kernel();
   constexpr int kThreads = 128;
@@ -556,7 +557,7 @@ template <typename T, int D, int W> __global__ void __launch_bounds__(128) ob_ca
   const int seq = c - 1;
   if (seq < 0 || (bad && starts.left_out(seq))) return;
   const int q0 = b.q_start[seq], q1 = b.q_start[seq + 1], kv = b.kv_len[seq], n = q1 - q0;
-  if (n <= 0 || kv <= 0) return;
+  if (n < a.least_new || n > a.most_new || kv <= 0) return;
   const int before = kv - n, mine = slot - (q0 / kPageTokens + seq), slots = q1 / kPageTokens + 1 - q0 / kPageTokens;
   const Rotation& r = a.rot;
   for (int64_t block = max(before, 0) / kPageTokens + mine; block * kPageTokens < kv; block += slots) {
@@ -669,14 +670,24 @@ cudaError_t launch_cache_append(const CacheAppendCall& c, cudaStream_t stream) {
   const bool wide = wide_rotation(c.rotary_dim, c.interleaved) && wide_rows(c.k, c.k_ts, c.k_hs) && wide_rows(c.v, c.v_ts, c.v_hs) &&
                     wide_rows(c.q, c.q_ts, c.q_hs) && wide_rows(c.q_out, c.qo_ts, c.qo_hs);
   const int64_t items = (int64_t)a.page_slots * a.kv_heads;
-  // Few tokens a sequence on average: a warp's rolled loops. Measured for 64 sequences of 1 / 2 / 4 / 8 tokens, 8 heads of 128
-  // with 32 query heads: 6.2 / 9.2 / 15.4 / 27.8 us, against 13.4 / 14.1 / 12.5 / 15.3 us.
-  const bool few = c.tokens <= 2 * c.seqs;
-  const int64_t blocks = few ? (items + 3) / 4 + (q.tokens + kFewTokens - 1) / kFewTokens : items + (q.tokens + kAppendTokens - 1) / kAppendTokens;
+  // Sequences of up to three tokens: a warp's rolled loops. Measured for 64 sequences of 1 / 2 / 3 / 4 / 8 tokens, 8 heads of 128
+  // with 32 query heads: 5.8 / 9.5 / 12.7 / 16.8 / 27.8 us, against 13.4 / 14.1 / 18.3 / 12.0 / 15.3 us; a page of 64 takes its warp 200.
+  // So the caller's bound decides, not the mean: where some sequences are longer and most are short, both kernels run, each for
+  // its sequences (255 single tokens and 200 for one more: 21.5 us, 217 in the warps alone; 1024 and 1000: 64 us, 283).
+  constexpr int kMostFew = 3, kAny = 0x7fffffff;
+  const bool short_ones = c.max_new <= kMostFew, both = !short_ones && c.tokens <= 2 * c.seqs;
+  a.least_new = 1, a.most_new = both ? kMostFew : kAny;
   auto go = [&](auto t, auto d, auto w) {
     constexpr int kDim = decltype(d)::value, kWidth = decltype(w)::value;
     using T = decltype(t);
-    if (few) return launch_following(ob_cache_append_few_kernel<T, kDim, kWidth>, dim3((unsigned)blocks), 128, 0, stream, a, q);
+    if (short_ones || both) {
+      const int64_t blocks = (items + 3) / 4 + (q.tokens + kFewTokens - 1) / kFewTokens;
+      const cudaError_t e = launch_following(ob_cache_append_few_kernel<T, kDim, kWidth>, dim3((unsigned)blocks), 128, 0, stream, a, q);
+      if (e != cudaSuccess || !both) return e;
+      a.least_new = kMostFew + 1, a.most_new = kAny;
+      q.tokens = 0;                                             // the queries are turned
+    }
+    const int64_t blocks = items + (q.tokens + kAppendTokens - 1) / kAppendTokens;
     return launch_following(ob_cache_append_kernel<T, kDim, kWidth>, dim3((unsigned)blocks), 2 * kDim, 0, stream, a, q);
   };
   auto by_width = [&](auto t, auto d) {

@@ -214,7 +214,7 @@ std::tuple<int64_t, int64_t> check_batch(const Tensor& q_start, const Tensor& kv
 }
 
 py::object cache_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& k_scale, const Tensor& v_scale,
-                        const Tensor& q_start, const Tensor& kv_len, const Tensor& table, const OptTensor& q_, const OptTensor& inv_freq_,
+                        const Tensor& q_start, const Tensor& kv_len, const Tensor& table, int64_t max_new, const OptTensor& q_, const OptTensor& inv_freq_,
                         const std::string& layout, double magnitude, const OptTensor& q_out_) {
   const Tensor *q = ptr(q_), *inv_freq = ptr(inv_freq_), *q_out = ptr(q_out_);
   const int code = type_code(k);
@@ -242,11 +242,11 @@ py::object cache_append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
   if (tokens > 0) {
     const Tensor k1 = inner_contiguous(k), v1 = inner_contiguous(v);
     c10::cuda::CUDAGuard guard(k.device());
-    check_rc(onebit_cache_append(k1.data_ptr(), k1.stride(0), k1.stride(1), v1.data_ptr(), v1.stride(0), v1.stride(1), q ? q1.data_ptr() : nullptr, q ? q1.stride(0) : 0,
+    check_rc(onebit_cache_append_ex(k1.data_ptr(), k1.stride(0), k1.stride(1), v1.data_ptr(), v1.stride(0), v1.stride(1), q ? q1.data_ptr() : nullptr, q ? q1.stride(0) : 0,
                                  q ? q1.stride(1) : 0, q ? y.data_ptr() : nullptr, q ? y.stride(0) : 0, q ? y.stride(1) : 0,
                                  static_cast<const double*>(data(inv_freq)), rotary_dim, inter, (float)magnitude, k_pages.data_ptr(), v_pages.data_ptr(),
                                  k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), k_pages.size(0), q_start.data_ptr<int>(), kv_len.data_ptr<int>(),
-                                 table.data_ptr<int>(), table.stride(0), table.size(1), tokens, table.size(0), heads, H, D, code, stream_of(k)));
+                                 table.data_ptr<int>(), table.stride(0), table.size(1), tokens, table.size(0), heads, H, D, max_new, code, stream_of(k)));
   }
   return q ? py::cast(y) : py::none();
 }

@@ -237,7 +237,9 @@ class CachedDecoder:
         self.kv_len.add_(start.diff())
         if not x.shape[0]:
             return x.new_empty(x.shape)
-        batch = block_ops.CacheBatch(start, self.kv_len, self.table, max_new=max(lengths))
+        # as wide as the longest sequence needs: attention deals out its work, and cuts a long cache into parts, by the table's width
+        width = -(-max(self.lengths) // block_ops.PAGE_TOKENS)
+        batch = block_ops.CacheBatch(start, self.kv_len, self.table[:, :width], max_new=max(lengths))
         with torch.no_grad():
             return self.model(x, self.caches, batch)
 

@@ -1,8 +1,30 @@
 """`CachedLlamaStack` and `CachedDecoder` on the host (no GPU)."""
+import pytest
 import torch
 import torch.nn as nn
 
-from onebitsparsemul_b200.decode_loop import CachedLlamaStack
+from onebitsparsemul_b200 import build
+from onebitsparsemul_b200.decode_loop import CachedDecoder, CachedLlamaStack
+
+
+@pytest.fixture(scope="module", autouse=True)
+def extension():
+    build.build_torch_extension()
+
+
+class Stub(nn.Module):
+    """A model that keeps the batches that it was called with."""
+
+    def __init__(self, hidden=8):
+        super().__init__()
+        self.hidden, self.batches = hidden, []
+
+    def make_caches(self, pages, device):
+        return []
+
+    def forward(self, x, caches, batch):
+        self.batches.append((batch, batch.kv_len.tolist()))
+        return x
 
 
 def small(**kw):
@@ -24,3 +46,14 @@ def test_frequencies_stay_in_64_bits():
     other.load_state_dict(small().half().state_dict())
     assert torch.equal(other.inv_freq, want)
     assert small().to("meta").inv_freq.device.type == "meta"
+
+
+def test_a_prompt_s_table_is_as_wide_as_its_longest_sequence():
+    model = Stub()
+    dec = CachedDecoder(model, 3, 32768, device="cpu")
+    for lengths, width in (([5, 64, 0], 1), ([0, 1, 0], 2), ([3, 0, 2000], 32), ([0, 0, 48], 32), ([1, 1, 1], 33), ([0, 30000, 0], 470)):
+        dec.prompt(torch.zeros(sum(lengths), 8), lengths)
+        batch, kv_len = model.batches[-1]
+        assert (batch.seqs, batch.width) == (3, width) and tuple(batch.block_table.shape) == (3, width)
+        assert kv_len == dec.lengths and max(kv_len) <= 64 * width
+        assert torch.equal(batch.block_table, dec.table[:, :width])

@@ -220,53 +220,70 @@ class CachedDecoder:
         self.step_batch = block_ops.CacheBatch(torch.arange(sequences + 1, **i32), self.kv_len, self.table, max_new=1)
         self.graph = None
 
-    def _grow(self, new):
+    def _grown(self, new):
+        """The lengths with `new` tokens more, or a refusal."""
         if len(new) != self.sequences or min(new) < 0 or any(a + b > self.max_len for a, b in zip(self.lengths, new)):
             raise ValueError(f"{new} new tokens do not fit {self.sequences} sequences of at most {self.max_len} that hold {self.lengths}")
-        self.lengths = [a + b for a, b in zip(self.lengths, new)]
+        return [a + b for a, b in zip(self.lengths, new)]
+
+    def _grow(self, new):
+        self.lengths = self._grown(new)
 
     def prompt(self, x, lengths):
-        """x (sum(lengths), hidden): the sequences' new tokens one after the other. Returns (tokens, hidden)."""
+        """x (sum(lengths), hidden): the sequences' new tokens one after the other. Returns (tokens, hidden). A call that raises
+        leaves the sequences as long as they were."""
         lengths = [int(n) for n in lengths]
-        if x.shape[0] != sum(lengths):
-            raise ValueError(f"{x.shape[0]} tokens for lengths {lengths}")
-        self._grow(lengths)
+        if tuple(x.shape) != (sum(lengths), self.model.hidden):
+            raise ValueError(f"x of {tuple(x.shape)} for lengths {lengths} and a hidden size of {self.model.hidden}")
+        grown = self._grown(lengths)
+        if not x.shape[0]:
+            return x.new_empty(x.shape)
         start = torch.zeros(self.sequences + 1, dtype=torch.int32)
         start[1:] = torch.tensor(lengths).cumsum(0)
         start = start.to(self.device)
-        self.kv_len.add_(start.diff())
-        if not x.shape[0]:
-            return x.new_empty(x.shape)
+        kv_len = self.kv_len + start.diff()
         # as wide as the longest sequence needs: attention deals out its work, and cuts a long cache into parts, by the table's width
-        width = -(-max(self.lengths) // block_ops.PAGE_TOKENS)
-        batch = block_ops.CacheBatch(start, self.kv_len, self.table[:, :width], max_new=max(lengths))
+        width = -(-max(grown) // block_ops.PAGE_TOKENS)
+        batch = block_ops.CacheBatch(start, kv_len, self.table[:, :width], max_new=max(lengths))
         with torch.no_grad():
-            return self.model(x, self.caches, batch)
+            y = self.model(x, self.caches, batch)
+        self.kv_len.copy_(kv_len)
+        self.lengths = grown
+        return y
 
     def _step(self):
         self.kv_len.add_(1)
         return self.model(self.x, self.caches, self.step_batch)
 
-    def step(self, x):
-        """x (sequences, hidden): one token for every sequence."""
-        if tuple(x.shape) != (self.sequences, self.model.hidden):
-            raise ValueError(f"x must be ({self.sequences}, {self.model.hidden})")
-        self._grow([1] * self.sequences)
-        if self.graph is None:
-            # The first calls load kernels and mark the packed weights as long-lived: they run outside the capture, on the
-            # sequences as they are, and the lengths are put back. What they wrote, the step itself writes again.
-            self.x = x.clone()
-            side = torch.cuda.Stream(device=self.device)
-            side.wait_stream(torch.cuda.current_stream(self.device))
+    def _capture(self, x):
+        """The graph of a step. The first calls load kernels and mark the packed weights as long-lived: they run outside the capture, on
+        the sequences as they are, and the lengths are put back. What they wrote, the step itself writes again."""
+        self.x = x.clone()
+        before = self.kv_len.clone()
+        side = torch.cuda.Stream(device=self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        try:
             with torch.cuda.stream(side), torch.no_grad():
                 for _ in range(2):
                     self._step()
-                    self.kv_len.sub_(1)
+                    self.kv_len.copy_(before)
+        finally:
             torch.cuda.current_stream(self.device).wait_stream(side)
+            self.kv_len.copy_(before)
             torch.cuda.synchronize(self.device)
-            self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph), torch.no_grad():
-                self.y = self._step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():
+            self.y = self._step()
+        self.graph = graph
+
+    def step(self, x):
+        """x (sequences, hidden): one token for every sequence. A call that raises leaves the sequences as long as they were."""
+        if tuple(x.shape) != (self.sequences, self.model.hidden):
+            raise ValueError(f"x must be ({self.sequences}, {self.model.hidden})")
+        grown = self._grown([1] * self.sequences)
+        if self.graph is None:
+            self._capture(x)
         self.x.copy_(x)
         self.graph.replay()
+        self.lengths = grown
         return self.y

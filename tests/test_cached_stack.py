@@ -57,3 +57,49 @@ def test_a_prompt_s_table_is_as_wide_as_its_longest_sequence():
         assert (batch.seqs, batch.width) == (3, width) and tuple(batch.block_table.shape) == (3, width)
         assert kv_len == dec.lengths and max(kv_len) <= 64 * width
         assert torch.equal(batch.block_table, dec.table[:, :width])
+
+
+class Failing(Stub):
+    fails = False
+
+    def forward(self, x, caches, batch):
+        if self.fails:
+            raise RuntimeError("out of memory")
+        return super().forward(x, caches, batch)
+
+
+def test_a_prompt_that_raises_leaves_the_sequences_as_they_were():
+    model = Failing()
+    dec = CachedDecoder(model, 2, 100, device="cpu")
+    dec.prompt(torch.zeros(7, 8), [3, 4])
+    model.fails = True
+    with pytest.raises(RuntimeError):
+        dec.prompt(torch.zeros(2, 8), [1, 1])
+    for x, lengths in ((torch.zeros(2, 9), [1, 1]), (torch.zeros(2, 8), [1, 2]), (torch.zeros(2), [1, 1]), (torch.zeros(200, 8), [100, 100]), (torch.zeros(2, 8), [3, -1])):
+        with pytest.raises(ValueError):
+            dec.prompt(x, lengths)
+    assert dec.lengths == dec.kv_len.tolist() == [3, 4]
+    model.fails = False
+    dec.prompt(torch.zeros(2, 8), [1, 1])
+    assert dec.lengths == dec.kv_len.tolist() == model.batches[-1][1] == [4, 5]
+    assert dec.prompt(torch.zeros(0, 8), [0, 0]).shape == (0, 8) and dec.lengths == [4, 5]
+
+
+@pytest.mark.gpu
+def test_a_step_that_raises_leaves_the_sequences_as_they_were():
+    class Once(Failing):
+        calls = 0
+
+        def forward(self, x, caches, batch):
+            self.calls += 1
+            if self.calls == 2:
+                raise RuntimeError("out of memory")
+            return x + batch.kv_len[:, None]
+    model = Once()
+    dec = CachedDecoder(model, 2, 100)
+    with pytest.raises(RuntimeError):
+        dec.step(torch.zeros(2, 8, device="cuda"))
+    assert dec.graph is None and dec.lengths == dec.kv_len.tolist() == [0, 0]
+    for i in range(3):
+        y = dec.step(torch.full((2, 8), 10.0 * i, device="cuda"))
+        assert (y == 10.0 * i + i + 1).all() and dec.lengths == dec.kv_len.tolist() == [i + 1] * 2

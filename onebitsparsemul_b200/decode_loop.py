@@ -272,7 +272,7 @@ class CachedDecoder:
             self.kv_len.copy_(before)
             torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph), torch.no_grad():
+        with torch.cuda.graph(graph, stream=side), torch.no_grad():        # this device's stream, whichever is current
             self.y = self._step()
         self.graph = graph
 

@@ -23,8 +23,8 @@ class Stub(nn.Module):
         return []
 
     def forward(self, x, caches, batch):
-        self.batches.append((batch, batch.kv_len.tolist()))
-        return x
+        self.batches.append((batch, None if x.is_cuda else batch.kv_len.tolist()))
+        return x + 0
 
 
 def small(**kw):
@@ -103,3 +103,19 @@ def test_a_step_that_raises_leaves_the_sequences_as_they_were():
     for i in range(3):
         y = dec.step(torch.full((2, 8), 10.0 * i, device="cuda"))
         assert (y == 10.0 * i + i + 1).all() and dec.lengths == dec.kv_len.tolist() == [i + 1] * 2
+
+
+@pytest.mark.gpu
+def test_a_step_is_captured_on_its_device_s_stream(monkeypatch):
+    """Without a stream of its own a capture takes one of the device that was current when the first graph of the process was made."""
+    seen, real = [], torch.cuda.graph
+
+    def graph(*args, stream=None, **kw):
+        seen.append(stream)
+        return real(*args, stream=stream, **kw)
+    monkeypatch.setattr(torch.cuda, "graph", graph)
+    device = torch.cuda.device_count() - 1
+    dec = CachedDecoder(Stub(), 2, 100, device=f"cuda:{device}")
+    for i in range(2):
+        assert (dec.step(torch.full((2, 8), float(i), device=dec.device)) == i).all()
+    assert [s.device.index for s in seen] == [device] and dec.kv_len.tolist() == [2, 2]

@@ -197,17 +197,17 @@ __global__ void __launch_bounds__(DecodeCfg<NT>::kThreads, 2) ob_gemm_decode_ker
       if (rows_contiguous) {
         // token j is contiguous along k: 16 pieces of 8 values per tile
         const int j = idx / (KL * 16), pc = idx % (KL * 16);
-        if (j < nvalid && (pc >> 4) < ntile) tv[i] = __ldg(reinterpret_cast<const uint4*>(a.b + (n0 + j) * a.k + k0 + pc * 8));
+        if (j < nvalid && (pc >> 4) < ntile) tv[i] = *reinterpret_cast<const uint4*>(a.b + (n0 + j) * a.k + k0 + pc * 8);
       } else {
         const int kk = idx / NT, pc = idx % NT;               // k-row of the round, 8-token piece of that row
         if ((kk >> 7) < ntile) {
           if (vec_rows) {
-            tv[i] = __ldg(reinterpret_cast<const uint4*>(a.b + (k0 + kk) * a.n + n0 + pc * 8));
+            tv[i] = *reinterpret_cast<const uint4*>(a.b + (k0 + kk) * a.n + n0 + pc * 8);
           } else if (quad_rows) {
             uint2* h4 = reinterpret_cast<uint2*>(&tv[i]);     // n % 4 == 0: whole groups of four tokens
 #pragma unroll
             for (int q4 = 0; q4 < 2; ++q4)
-              if (8 * pc + 4 * q4 < nvalid) h4[q4] = __ldg(reinterpret_cast<const uint2*>(a.b + (k0 + kk) * a.n + n0 + 8 * pc + 4 * q4));
+              if (8 * pc + 4 * q4 < nvalid) h4[q4] = *reinterpret_cast<const uint2*>(a.b + (k0 + kk) * a.n + n0 + 8 * pc + 4 * q4);
           } else {
             __half* h = reinterpret_cast<__half*>(&tv[i]);
 #pragma unroll

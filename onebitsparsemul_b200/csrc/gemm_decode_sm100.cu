@@ -293,12 +293,12 @@ __global__ void __launch_bounds__(kThreads, 2) ob_gemm_fewtok_kernel(const __gri
       if ((int)(tplace[i] >> 24) < ntile) {
         const __half* src = a.b + tsrc[i];
         if (kmajor || vec_rows) {
-          tv[i] = __ldg(reinterpret_cast<const uint4*>(src));
+          tv[i] = *reinterpret_cast<const uint4*>(src);
         } else if (quad_rows) {
           const int ng = piece_index(i) % NG;
           uint2* h4 = reinterpret_cast<uint2*>(&tv[i]);       // n % 4 == 0: whole groups of four tokens
-          h4[0] = __ldg(reinterpret_cast<const uint2*>(src));
-          if (8 * ng + 4 < nvalid) h4[1] = __ldg(reinterpret_cast<const uint2*>(src + 4));
+          h4[0] = *reinterpret_cast<const uint2*>(src);
+          if (8 * ng + 4 < nvalid) h4[1] = *reinterpret_cast<const uint2*>(src + 4);
         } else {
           const int ng = piece_index(i) % NG;
           __half* h = reinterpret_cast<__half*>(&tv[i]);

@@ -24,3 +24,10 @@ def test_kernels_that_start_early_have_no_read_only_loads(name):
         assert not re.search(r"__ldg|ld\.global\.nc|__ldcs|__ldca|__restrict__", k)
     if all("follow_previous_kernel()" in k for k in kernels if "__global__" in k):      # then the helpers are theirs too
         assert not re.search(r"__ldg|ld\.global\.nc|__ldcs|__ldca|__restrict__", code)
+
+
+@pytest.mark.parametrize("name", ["gemm_decode.cu", "gemm_decode_sm100.cu"])
+def test_few_token_products_read_tokens_that_may_just_have_been_written(name):
+    """They start before the norm that writes their tokens is complete."""
+    code = code_of(name)
+    assert "griddepcontrol.wait" in code and not re.search(r"__ldg|ld\.global\.nc|__ldcs|__ldca|__restrict__", code)

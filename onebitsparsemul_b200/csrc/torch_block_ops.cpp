@@ -79,6 +79,9 @@ void check_output(const Tensor& out, const char* name, std::initializer_list<con
   for (const Tensor* t : apart) TORCH_CHECK_VALUE(!t || !ob_overlap::may_overlap(place, place_of(*t)), name, " overlaps an input");
 }
 
+// a scalar as the kernels get it
+bool finite32(double v) { return std::isfinite((float)v); }
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // t as (rows, hidden) with contiguous rows
@@ -98,7 +101,7 @@ py::object residual_norm(const Tensor& x, const Tensor& weight, const OptTensor&
   const auto like_x = [&](const Tensor& t) { return t.sizes() == x.sizes(); };
   TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type() && channel(weight), "weight must be (", hidden, ",) of x's type");
   TORCH_CHECK_VALUE(!post || (post->scalar_type() == x.scalar_type() && channel(*post)), "post_weight must be (", hidden, ",) of x's type");
-  TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0 && std::isfinite(residual_scale), "eps must be finite and not negative, residual_scale finite");
+  TORCH_CHECK_VALUE(finite32(eps) && eps >= 0 && finite32(residual_scale), "eps must be finite and not negative, residual_scale finite (in 32 bits)");
   Tensor h, r2;
   if (!residual) {
     TORCH_CHECK_VALUE(!gate && !post && !residual_out && residual_scale == 1.0, "gate, post_weight, residual_scale and residual_out need a residual");
@@ -168,6 +171,7 @@ Tensor rotary_tokens(const Tensor& x, const Tensor& positions, const Tensor& inv
   const bool wide = positions.scalar_type() == torch::kLong;
   TORCH_CHECK_VALUE((wide || positions.scalar_type() == torch::kInt) && positions.dim() == 1 && positions.size(0) == tokens, "positions must be (tokens,) int32 or int64");
   const bool inter = interleaved_layout(layout);
+  TORCH_CHECK_VALUE(finite32(magnitude), "magnitude must be finite (in 32 bits)");
   const int rotary_dim = rotary_dim_of(inv_freq, dim);
   if (out) check_turned(*out, x, "out", {&positions, &inv_freq});
   Tensor y = out ? *out : torch::empty(x.sizes(), x.options());
@@ -225,6 +229,7 @@ py::object cache_append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
   TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type() && (!q || q->scalar_type() == k.scalar_type()), "q, k and v must have one type");
   TORCH_CHECK_VALUE(tokens <= (1 << 24), "at most 2^24 tokens");
   const bool inter = interleaved_layout(layout);
+  TORCH_CHECK_VALUE(finite32(magnitude), "magnitude must be finite (in 32 bits)");
   const int rotary_dim = inv_freq ? rotary_dim_of(*inv_freq, D) : 0;
   int64_t heads = H;
   Tensor y, q1;
@@ -262,7 +267,7 @@ Tensor cache_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   TORCH_CHECK_VALUE(heads % H == 0 && heads >= 1 && heads <= 4096, heads, " query heads are no multiple of ", H, " cache heads");
   TORCH_CHECK_VALUE(tokens <= (1 << 24), "at most 2^24 tokens");
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)D);
-  TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
+  TORCH_CHECK_VALUE(finite32(scale), "scale must be finite (in 32 bits)");
   const auto aligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; };
   TORCH_CHECK_VALUE(!out || (out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->is_contiguous() && aligned(*out)),
                     "out must be contiguous (and 16-byte aligned) with q's shape and type");

@@ -236,7 +236,7 @@ int onebit_rotary(const void *x, int64_t x_token_stride, int64_t x_head_stride, 
  * at most 448, but not less than the scale of tokens that the page held before the call; those are re-scaled if it grew. A page
  * without earlier tokens gets zeros behind the new ones. Infinities are stored as the largest value, a NaN key value as NaN; a
  * token with a NaN in v has it stored as 0 and its key made NaN. q (nullable, heads a multiple of kv_heads) is turned into q_out,
- * which may be q. A page that is written may belong to one sequence of the batch only. */
+ * which may be q. A page that is written stands once in the batch's table. */
 int onebit_cache_append(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
                         const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out, int64_t q_out_token_stride, int64_t q_out_head_stride,
                         const double *inv_freq, int rotary_dim, int interleaved, float magnitude, void *k_pages, void *v_pages,

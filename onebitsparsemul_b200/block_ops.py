@@ -168,8 +168,8 @@ def cache_append(k, v, cache, batch, q=None, inv_freq=None, layout="half", magni
     The scale of a page and head is the smallest power of two (2^-32 to 2^32) that brings the largest finite |value| of its
     tokens into e4m3's range; when a step's tokens make it grow, the page's earlier tokens are re-scaled. Infinities are
     stored as the largest value of the page's scale. A NaN key stays NaN; a token with a NaN value has it stored as 0 and its key
-    made NaN, so that the queries that see the token answer NaN and no others. A page that a step writes must belong to one
-    sequence of the batch only."""
+    made NaN, so that the queries that see the token answer NaN and no others. A page that a step writes must stand once in the
+    batch's table: in one sequence, in one place."""
     return _ext().cache_append(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, batch.q_start, batch.kv_len, batch.block_table,
                                batch.max_new, q, inv_freq, layout, magnitude, q_out)
 
@@ -178,7 +178,7 @@ def cache_attend(q, cache, batch, scale=None, causal=True, out=None):
     """softmax(scale * q k^T) v of the step's queries q (tokens, heads, head_dim) over their sequences' cached tokens
     (``onebit_cache_attend``); call it after `cache_append` of the same batch. Query head h reads cache head
     h // (heads // kv_heads). causal: a token sees the positions up to its own (the new tokens are the last ones of the
-    sequence), else the whole sequence. scale: head_dim ** -0.5 by default. A row that sees nothing is zero. `out`: contiguous,
-    q's shape and type."""
+    sequence), else the whole sequence. scale: head_dim ** -0.5 by default. A row that sees nothing, or nothing but scores of
+    minus infinity, is zero. `out`: contiguous, q's shape and type, apart from q and the cache."""
     return _ext().cache_attend(q, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, batch.q_start, batch.kv_len, batch.block_table,
                                batch.max_new, scale, causal, out)

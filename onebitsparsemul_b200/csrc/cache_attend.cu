@@ -682,12 +682,13 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256) o
 }
 
 // Which kernel has which sequences (the times: contexts of 4096, 32 / 8 heads of 128, this file's kernel / the tensor-memory
-// kernel). A row tile of 16 here costs a quarter of one of 256 there: 16 sequences of 8 / 16 / 24 tokens take 46 / 92, 89 / 90 and
-// 131 / 95 us, so up to 64 rows per cache head are this file's. So are sequences of up to 256 rows that have as few on the mean
-// (64 single tokens and one sequence of 64: 132 / 298 us), or that leave half the GPU free (one of 32 tokens: 17 / 33 us).
-// A longer bound far above the mean is that of a prompt among single tokens. Where the sequences are enough to fill the GPU on
-// their own, both kernels run, each for its sequences: n single tokens and a prompt of 512 take, so / in the prompt's kernel
-// alone, 92 / 141 us for n = 14 and 172 / 307 us for n = 64. Fewer hide behind the prompt's tiles.
+// kernel). A row tile of 16 here costs about a quarter of one of 256 there, so up to 64 rows per cache head are this file's:
+// 16 sequences of 8 / 16 / 24 tokens take 48 / 88, 92 / 80 and 136 / 81 us, 64 of 8 / 16 171 / 302 and 315 / 305 us; over contexts of
+// 512, and with 4 or 8 sequences, 16 tokens are better off here (17 / 18, 29 / 41 and 47 / 64 us). So are sequences of up to 256 rows
+// that have as few on the mean (64 single tokens and one sequence of 64: 136 / 299 us), or that leave half the GPU free (one of 32
+// tokens: 17 / 25 us). A longer bound far above the mean is that of a prompt among single tokens. Where the sequences are enough to
+// fill the GPU on their own, both kernels run, each for its sequences: n single tokens and a prompt of 512 take, so / in the
+// prompt's kernel alone, 113 / 150 us for n = 14 and 174 / 310 us for n = 64. Fewer hide behind the prompt's tiles.
 constexpr int kFewRows = 64, kFewRowsMost = 256;
 struct Plan { bool few, many; int few_rows; };
 Plan plan_of(const ob::CacheAttendCall& c) {

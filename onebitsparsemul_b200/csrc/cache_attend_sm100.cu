@@ -17,7 +17,7 @@
 //     would be missing where one token has nearly all the weight and its page is louder than the others.
 // Scales as in cache_attend.cu: the key scale multiplies the score, the value scale goes into the exponent.
 // Long caches with too few row tiles to fill the chip are split along the cached tokens; the parts are joined by a second kernel.
-// Measured: a prompt of 8192, 32 / 8 heads of 128, 592 us (930 TFLOP/s of the causal half, 56 % of the cuBLAS rate). No unit is
+// Measured: a prompt of 8192, 32 / 8 heads of 128, 600 us (916 TFLOP/s of the causal half, 55 % of the cuBLAS rate). No unit is
 // saturated: the softmax's instructions and the widening share the issue slots and wait for each other (leaving out either, or
 // the products, changes the time by 2 to 8 %).
 // Every mbarrier wait is bounded. No TMA.
@@ -562,9 +562,10 @@ int64_t many_slots(const ob::CacheAttendCall& c) { return c.tokens * (c.heads / 
 
 // Parts that the cache is cut into, for row tiles too few to fill the GPU: the number with the least estimated time, from what
 // was measured for heads of 128 values: 2.3 us a step of 128 tokens (64 values: 1.95), 11 us a CTA besides, and for the join 4 us
-// and the partial results at 1.7 TB/s. 32 / 8 heads, in 1 / 2 / 4 / 8 parts: 512 tokens over 4096 85 / 60 / 77 / 109 us (2 taken),
-// 128 over 4096 85 / 55 / 40 / 34 (8), 2048 over 2048 58 / 118 / 181 / 299 (1), 3 x 512 over 16384 598 / 503 / 551 / 619 (2; in 3
-// 472).
+// and the partial results at 1.7 TB/s. 32 / 8 heads, in 1 / 2 / 4 / 8 parts: 512 tokens over 4096 86 / 63 / 79 / 111 us (2 taken),
+// 128 over 4096 86 / 56 / 39 / 33 (8), 2048 over 2048 58 / 123 / 187 / 307 (1), 3 x 512 over 16384 604 / 510 / 557 / 622 (2; the
+// estimate misses 3 parts there, 482 us, by 6 %). It counts the table's width for every sequence: a table much wider than the
+// batch's longest sequence is cut too often (2048 tokens in a table of 32768: 159 us), so callers pass a table as wide as they need.
 int many_splits(const ob::CacheAttendCall& c) {
   const int64_t group = c.heads / c.kv_heads, sms = ob::sm_count(), steps = (c.table_width + 1) / 2;
   const int64_t ctas = ((c.tokens * group + kCtaRows - 1) / kCtaRows + (c.seqs - 1) / 2) * c.kv_heads;

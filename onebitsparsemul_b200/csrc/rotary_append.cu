@@ -215,7 +215,7 @@ __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b, __nv_bfloat
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 // 2 D threads: 16 groups of 4 tokens (a word of the transposed values) x D / 8 groups of 8 values. The grid is in two halves:
-// 8 prompts of up to 2048 tokens (8 heads of 128, 32 query heads) take 43.7 us, of which the queries alone are 30 (the rate of the
+// 8 prompts of up to 2048 tokens (8 heads of 128, 32 query heads) take 44.1 us, of which the queries alone are 30 (the rate of the
 // rotation by itself) and the pages' instructions the rest; the pages among the queries instead of before them: 44.9 us. At 80
 // registers three CTAs of 256 threads share an SM and a thread has all kBatch pieces of 4 tokens' queries under way; four CTAs at
 // 64 registers spill (49.2 us, with two tokens 46.7), two at 128 are too few (50.3 us).
